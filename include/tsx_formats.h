@@ -28,6 +28,9 @@ extern "C" {
 #endif
 
 enum {
+    TSX_F32 = 0, /* plain values: router logits and adapter matrices */
+    TSX_F16 = 1,
+    TSX_BF16 = 30,
     TSX_Q4_0 = 2,
     TSX_Q8_0 = 8,
     TSX_Q8_1 = 9,

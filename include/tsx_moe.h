@@ -195,15 +195,15 @@ TSX_API int tsx_moe_group_resident(const int32_t* ids, int n_ent, int k, int n_e
 TSX_API int tsx_moe_merge_rows(float* parts, const float* rows, const int32_t* miss, int n_ent, int64_t n,
                                void* stream);
 /* The prompt's entries sorted by expert: bounds[x]..bounds[x+1] are expert x's sorted rows (n_expert + 1 ints);
- * sorted row r holds entry ent_dst[r] of token ent_tok[r]; rinv[e] = entry e's sorted row; *max_rows = the most
- * rows of one expert.  Rows inside an expert are in entry order.  All on the device (no host round trip).
+ * sorted row r holds entry ent_dst[r] of token ent_tok[r]; rinv[e] = entry e's sorted row (-1 for an
+ * id out of range, which has no row); *max_rows = the most rows of one expert.  Rows inside an expert are in entry order.  All on the device (no host round trip).
  * Replaces k_route_count / k_route_scan / k_route_scatter (src/qwen35/q36_engine.cu:483-510) and the
  * max_rows read back at src/qwen35/q36_engine.cu:2864-2869. */
 TSX_API int tsx_moe_route_sort(const int32_t* ids, int n_ent, int k, int n_expert, int32_t* bounds, int32_t* ent_dst,
                                int32_t* ent_tok, int32_t* rinv, int32_t* max_rows, void* stream);
 /* x[t] += w[t][0]*parts[p(t,0)] then fmaf(w[t][j], parts[p(t,j)], .) in pick order, + sigmoid(sgate[t*sg_stride])
  * * shared[t] (shared/sgate may be null); p(t,j) = prow ? prow[t*k+j] : t*k+j.  n values per row.
- * Replaces k_moe_out / k_moe_out_small without the norm (src/qwen35/q36_engine.cu:304-332;
+ * A prow below 0 is an entry without a row: it adds nothing.  Replaces k_moe_out / k_moe_out_small without the norm (src/qwen35/q36_engine.cu:304-332;
  * src/qwen35/q36_kernels.cuh:248-290). */
 TSX_API int tsx_moe_combine(float* x, const float* parts, const int32_t* prow, const float* wts, int k,
                             const float* shared, const float* sgate, int sg_stride, int n, int n_tok, void* stream);
@@ -214,6 +214,46 @@ TSX_API int tsx_moe_combine(float* x, const float* parts, const int32_t* prow, c
 TSX_API int tsx_moe_combine_norm(float* x, const float* parts, const int32_t* prow, const float* wts, int k,
                                  const float* shared, const float* sgate, int sg_stride, int n, int n_tok,
                                  const float* norm_w, float eps, float* h, void* hq, void* stream);
+
+/* Routing by the rules of several model families, beside tsx_moe_router_topk (softmax, fp32).  logits [n_tok][n_expert],
+ * rows `ld` values apart, of r->type -> ids [n_tok][k] and weights [n_tok][k]:
+ *   s_e = softmax over the experts, or 1 / (1 + exp(-l_e)); an expert whose logit is -inf or NaN takes no part (an expert
+ *         removed, a padded token), and a softmax over a logit of +inf has no picks
+ *   c_e = s_e + bias_e, or l_e without a bias: what the experts are picked by (an expert whose c is -inf or NaN never is)
+ *   n_group > 1: expert e is in group e / (n_expert / n_group); the topk_group groups of largest value keep their experts,
+ *         a group's value being its largest c (group_top 1) or the sum of its two largest s + bias (2; of one where only one
+ *         takes part)
+ *   the k largest c, ties to the lower id (of groups: to the lower group); where fewer are left, id -1 and weight 0
+ *   w_j = scale * s_j, divided by max(sum of the picks' s, floor) when norm is set
+ * The picks are those of exact arithmetic: c is formed in 64 bits.  prow (may be null) receives [n_tok][k] entry numbers
+ * t * k + j, -1 where the id is -1: tsx_moe_combine's rows in entry order.  counts (may be null) has the number of tokens
+ * that picked expert e added to counts[e].  n_expert 1..512, k 1..16, n_group 1..64 of equal size with k experts in those
+ * kept; n_tok * k below 2^31.  tsx_moe_group and tsx_moe_route_sort leave out entries of id -1. */
+enum { TSX_SCORE_SOFTMAX = 0, TSX_SCORE_SIGMOID = 1 };
+typedef struct {
+    int32_t type;  /* of the logits: TSX_F32, TSX_F16 or TSX_BF16 */
+    int32_t score; /* TSX_SCORE_* */
+    int32_t n_expert, k;
+    int32_t n_group, topk_group, group_top; /* 1, 1, 1 for no groups */
+    int32_t norm;
+    float scale, floor; /* floor > 0 (tsx_moe_router_topk's is 6.1035e-5) */
+    const float* bias;  /* device [n_expert], or null */
+} tsx_router;
+TSX_API int tsx_moe_route(const tsx_router* r, const void* logits, int64_t ld, int32_t* ids, float* weights,
+                          int32_t* prow, int32_t* counts, int n_tok, void* stream);
+/* The gradient of tsx_moe_route's weights: dweights [n_tok][k] of the picks ids -> dlogits [n_tok][n_expert] of r->type,
+ * rows ld_d values apart, every value written (0 for an expert that takes no part).  The choice itself has no gradient, nor
+ * has the bias.  An id below 0 or past the experts has no term; an expert named twice in a row gets both terms. */
+TSX_API int tsx_moe_route_backward(const tsx_router* r, const void* logits, int64_t ld, const int32_t* ids,
+                                   const float* dweights, void* dlogits, int64_t ld_d, int n_tok, void* stream);
+/* The gradients of tsx_moe_combine, dy [n_tok][n] that of its sum: dwts[t][j] = dy[t] . parts[p(t,j)],
+ * dparts[p(t,j)] = wts[t][j] * dy[t], dshared[t] = g * dy[t] and dsgate[t] = g (1 - g) dy[t] . shared[t] with
+ * g = sigmoid(sgate[t * sg_stride]).  Each of the four outputs may be null; dshared and dsgate go with shared.  dsgate is
+ * dense.  The entries' rows are distinct; an entry without a row (prow below 0) has dwts 0, and rows of dparts that no entry
+ * names are left as they are. */
+TSX_API int tsx_moe_combine_backward(const float* dy, const float* parts, const int32_t* prow, const float* wts, int k,
+                                     const float* shared, const float* sgate, int sg_stride, int n, int n_tok,
+                                     float* dwts, float* dparts, float* dshared, float* dsgate, void* stream);
 
 /* ------------------------------------------------------------------------------------------------ prefill */
 /* Bytes of `rows` activation rows of `cols` values quantized for tsx_moe_mmq_run.

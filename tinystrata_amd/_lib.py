@@ -15,6 +15,7 @@ TSX_OK, TSX_ERR_UNSUPPORTED, TSX_ERR_ARG, TSX_ERR_FORMAT, TSX_ERR_NOT_FOUND, TSX
 CPU_MAXT, POOL_MAX_SPLIT = 8, 96  # tokens per CPU job, experts per pool batch (include/tsx_pool.h)
 
 # type ids (ggml's)
+F32, F16, BF16 = 0, 1, 30
 Q4_0, Q8_0, Q8_1, Q4_K, Q6_K, Q8_K, IQ3_XXS, IQ3_S = 2, 8, 9, 12, 14, 15, 18, 21
 
 
@@ -74,6 +75,13 @@ class MmvqSlots(C.Structure):
     """tsx_mmvq_slots: up to 8 matrices given by the host (reference MmvqSlots)."""
 
     _fields_ = [("w", C.c_void_p * 8), ("x", C.c_void_p * 8), ("y", C.c_void_p * 8)]
+
+
+class RouterArgs(C.Structure):
+    """tsx_router: the rule by which tokens pick experts."""
+
+    _fields_ = [(n, C.c_int32) for n in ("type", "score", "n_expert", "k", "n_group", "topk_group", "group_top", "norm")
+                ] + [("scale", C.c_float), ("floor", C.c_float), ("bias", C.c_void_p)]
 
 
 class GgufTensor(C.Structure):
@@ -173,6 +181,9 @@ SIGNATURES = {
     "tsx_moe_decode_layer_noalloc_max_bytes": (SZ, []),
     "tsx_moe_decode_layer_noalloc": (I32, [C.POINTER(ExpertLayout), P, U64, I32, I32, I32, P, P, P, P, I32, P, P, P, P]),
     "tsx_moe_router_topk": (I32, [P, P, P, I32, I32, I32, P]),
+    "tsx_moe_route": (I32, [C.POINTER(RouterArgs), P, I64, P, P, P, P, I32, P]),
+    "tsx_moe_route_backward": (I32, [C.POINTER(RouterArgs), P, I64, P, P, P, I64, I32, P]),
+    "tsx_moe_combine_backward": (I32, [P, P, P, P, I32, P, P, I32, I32, I32, P, P, P, P, P]),
     "tsx_moe_group": (I32, [P, I32, I32, I32, P, U64, P, P, P, P, P, P]),
     "tsx_moe_group_resident": (I32, [P, I32, I32, I32, P, P, U64, P, P, P, P, P, P]),
     "tsx_moe_merge_rows": (I32, [P, P, P, I32, I64, P]),

@@ -31,6 +31,7 @@ SOURCES = [
     "tsx_decode.hip",
     "tsx_layer.hip",
     "tsx_route.hip",
+    "tsx_router.hip",
     "tsx_prefill.hip",
 ]
 

@@ -226,7 +226,15 @@ __global__ void __launch_bounds__(kSortThreads) route_sort_kernel(const int32_t*
         ent_dst[r] = e;
         ent_tok[r] = e / k;
         rinv[e] = r;
+    } else if (e < n_ent) {
+        rinv[e] = -1;  // an id out of range: the entry has no row
     }
+}
+
+// a part row's value, 0 for an entry without a row (prow < 0; the load goes to row 0, so that it needs no branch)
+__device__ __forceinline__ float part_value(float v, int row) { return row < 0 ? 0.f : v; }
+__device__ __forceinline__ float4 part_value(float4 v, int row) {
+    return row < 0 ? float4{0.f, 0.f, 0.f, 0.f} : v;
 }
 
 // x[t][i] += sum_j w_j parts[p(t,j)][i] (first product, then FMA, pick order) + sigmoid(sgate) * shared[t][i]
@@ -250,7 +258,10 @@ __global__ void __launch_bounds__(256) combine_kernel(float* __restrict__ x, con
     const int i = blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= n) return;
     const float* wr = wts + (int64_t) t * k;
-    auto part = [&](int j) { return parts[(int64_t) (prow ? prow[t * k + j] : t * k + j) * n + i]; };
+    auto part = [&](int j) {
+        const int row = prow ? prow[t * k + j] : t * k + j;
+        return part_value(parts[(int64_t) max(row, 0) * n + i], row);
+    };
     float acc = wr[0] * part(0);
     for (int j = 1; j < k; ++j) acc = __builtin_fmaf(wr[j], part(j), acc);
     if (shared) {
@@ -271,7 +282,8 @@ __global__ void __launch_bounds__(256) combine4_kernel(float* __restrict__ x, co
     if (i >= n) return;
     const float* wr = wts + (int64_t) t * k;
     auto part = [&](int j) {
-        return *(const float4*) (parts + (int64_t) (prow ? prow[t * k + j] : t * k + j) * n + i);
+        const int row = prow ? prow[t * k + j] : t * k + j;
+        return part_value(*(const float4*) (parts + (int64_t) max(row, 0) * n + i), row);
     };
     float4 p = part(0);
     const float w0 = wr[0];
@@ -308,15 +320,18 @@ __global__ void __launch_bounds__(kNormThreads) combine_norm_kernel(float* __res
     __shared__ const float* s_part[kNormMaxK];
     __shared__ float s_red[kNormThreads / 64];
     const int t = blockIdx.x, tid = threadIdx.x;
-    if (tid < k) s_part[tid] = parts + (int64_t) (prow ? prow[t * k + tid] : t * k + tid) * n;
+    if (tid < k) {
+        const int row = prow ? prow[t * k + tid] : t * k + tid;
+        s_part[tid] = row < 0 ? nullptr : parts + (int64_t) row * n;
+    }
     __syncthreads();
     const float* wr = wts + (int64_t) t * k;
     const float gs = shared ? 1.0f / (1.0f + expf(-sgate[(int64_t) t * sg_stride])) : 0.f;
     float* xr = x + (int64_t) t * n;
     float q = 0.f;
     for (int i = tid; i < n; i += kNormThreads) {
-        float acc = wr[0] * s_part[0][i];
-        for (int j = 1; j < k; ++j) acc = __builtin_fmaf(wr[j], s_part[j][i], acc);
+        float acc = wr[0] * (s_part[0] ? s_part[0][i] : 0.f);
+        for (int j = 1; j < k; ++j) acc = __builtin_fmaf(wr[j], s_part[j] ? s_part[j][i] : 0.f, acc);
         if (shared) acc += gs * shared[(int64_t) t * n + i];
         const float v = xr[i] + acc;
         xr[i] = v;
@@ -348,7 +363,8 @@ __global__ void __launch_bounds__(kNormThreads) combine_norm4_kernel(float* __re
     const float gs = shared ? 1.0f / (1.0f + expf(-sgate[(int64_t) t * sg_stride])) : 0.f;
     float* xr = x + (int64_t) t * n;
     auto part = [&](int j, int i) {
-        return *(const float4*) (parts + (int64_t) (prow ? prow[t * k + j] : t * k + j) * n + i);
+        const int row = prow ? prow[t * k + j] : t * k + j;
+        return part_value(*(const float4*) (parts + (int64_t) max(row, 0) * n + i), row);
     };
     for (int i = 4 * tid; i < n; i += 4 * kNormThreads) {
         const float4 xv = *(const float4*) (xr + i);

@@ -11,7 +11,8 @@ import ctypes as C
 import numpy as np
 import torch
 
-from ._lib import IQ3_S, IQ3_XXS, Q4_K, Q8_0, ExpertLayout, MmqProduct, MmvqIds, MmvqSlots, check, lib
+from ._lib import (BF16, F16, F32, IQ3_S, IQ3_XXS, Q4_K, Q8_0, ExpertLayout, MmqProduct, MmvqIds, MmvqSlots, RouterArgs,
+                   check, lib)
 
 WEIGHT_TYPES = (Q8_0, Q4_K, IQ3_XXS, IQ3_S)
 Q8_1_BLOCK_BYTES = 36
@@ -28,6 +29,44 @@ def _p(t: torch.Tensor | None) -> int | None:
 def _stream(stream=None) -> int:
     s = stream if stream is not None else torch.cuda.current_stream()
     return s.cuda_stream
+
+
+PLAIN_TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+
+
+def _expect(what: str, name: str, t: torch.Tensor | None, shape, dtype, like: torch.Tensor | None = None,
+            rows: bool = False) -> None:
+    """Refuses a tensor of another type, shape or device than the call takes (None stands for an absent one); `rows`:
+    rows may lie further apart than their length, else the tensor is dense."""
+    if t is None:
+        return
+    if t.dtype != dtype:
+        raise ValueError(f"{what}: {name} is {t.dtype}, not {dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, not {tuple(shape)}")
+    if like is not None and t.device != like.device:
+        raise ValueError(f"{what}: {name} is on {t.device}, not {like.device}")
+    if rows:
+        if t.numel() and ((t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
+            raise ValueError(f"{what}: {name}'s rows are not dense (strides {t.stride()})")
+    elif not t.is_contiguous():
+        raise ValueError(f"{what}: {name} is not contiguous")
+
+
+def _ld(t: torch.Tensor | None) -> int:
+    """Values between a matrix's rows (of a single row: its length)."""
+    return 0 if t is None else t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _launch(what: str, fn, like: torch.Tensor, stream, *args) -> None:
+    """fn(*args, stream) on like's device: on its current stream unless one is given."""
+    if not like.is_cuda:
+        raise ValueError("device tensors only")
+    if like.device.index == torch.cuda.current_device():
+        check(fn(*args, _stream(stream)), what)
+        return
+    with torch.cuda.device(like.device):
+        check(fn(*args, _stream(stream)), what)
 
 
 # ------------------------------------------------------------------ formats
@@ -155,6 +194,66 @@ def native_router_topk(logits: torch.Tensor, k: int, ids=None, weights=None, str
     return ids, weights
 
 
+class Router:
+    """The rule by which tokens pick experts (tsx_router): softmax or sigmoid scores, a bias added for the choice alone
+    (fp32 [n_expert], read at every call), the topk_group of n_group groups of experts kept (by the largest choice value
+    of a group, or the sum of its two largest), weights divided by their sum (at least `floor`) when norm is set, times
+    scale."""
+
+    SCORES = {"softmax": 0, "sigmoid": 1}
+
+    def __init__(self, n_expert: int, k: int, score: str = "softmax", bias: torch.Tensor | None = None, n_group: int = 1,
+                 topk_group: int = 1, group_top: int = 1, norm: bool = True, scale: float = 1.0,
+                 floor: float = 6.103515625e-5):
+        if score not in self.SCORES:
+            raise ValueError(f"Router: score {score!r} (softmax or sigmoid)")
+        _expect("Router", "bias", bias, (n_expert,), torch.float32)
+        self.n_expert, self.k, self.bias = n_expert, k, bias
+        self.args = {t: RouterArgs(type=code, score=self.SCORES[score], n_expert=n_expert, k=k, n_group=n_group,
+                                   topk_group=topk_group, group_top=group_top, norm=int(norm), scale=scale, floor=floor,
+                                   bias=_p(bias)) for t, code in PLAIN_TYPES.items()}
+
+    def args_for(self, what: str, logits: torch.Tensor) -> RouterArgs:
+        if logits.dim() != 2 or logits.dtype not in self.args:
+            raise ValueError(f"{what}: logits [n_tok, n_expert] in fp32, fp16 or bf16")
+        _expect(what, "logits", logits, (logits.shape[0], self.n_expert), logits.dtype, self.bias, rows=True)
+        return self.args[logits.dtype]
+
+
+def route(router: Router, logits: torch.Tensor, ids=None, wts=None, prow=None, counts=None, stream=None):
+    """The picked experts' ids [n_tok, k] int32 (-1 where none is left) and weights [n_tok, k]; logits rows may lie apart.
+    prow [n_tok, k] int32, if given: moe_combine's rows in entry order.  counts [n_expert] int32, if given: the tokens of
+    each expert are added."""
+    a = router.args_for("route", logits)
+    shape = (logits.shape[0], router.k)
+    if ids is None:
+        ids = torch.empty(shape, dtype=torch.int32, device=logits.device)
+    if wts is None:
+        wts = torch.empty(shape, dtype=torch.float32, device=logits.device)
+    _expect("route", "ids", ids, shape, torch.int32, logits)
+    _expect("route", "wts", wts, shape, torch.float32, logits)
+    _expect("route", "prow", prow, shape, torch.int32, logits)
+    _expect("route", "counts", counts, (router.n_expert,), torch.int32, logits)
+    _launch("route", lib().tsx_moe_route, logits, stream, C.byref(a), _p(logits), _ld(logits), _p(ids), _p(wts), _p(prow),
+            _p(counts), shape[0])
+    return ids, wts
+
+
+def route_backward(router: Router, logits: torch.Tensor, ids: torch.Tensor, dwts: torch.Tensor, dlogits=None,
+                   stream=None) -> torch.Tensor:
+    """The weights' gradient dwts [n_tok, k] of the picks ids -> the logits' [n_tok, n_expert], in the logits' type."""
+    a = router.args_for("route_backward", logits)
+    shape = (logits.shape[0], router.k)
+    if dlogits is None:
+        dlogits = torch.empty(tuple(logits.shape), dtype=logits.dtype, device=logits.device)
+    _expect("route_backward", "ids", ids, shape, torch.int32, logits)
+    _expect("route_backward", "dwts", dwts, shape, torch.float32, logits)
+    _expect("route_backward", "dlogits", dlogits, logits.shape, logits.dtype, logits, rows=True)
+    _launch("route_backward", lib().tsx_moe_route_backward, logits, stream, C.byref(a), _p(logits), _ld(logits), _p(ids),
+            _p(dwts), _p(dlogits), _ld(dlogits), shape[0])
+    return dlogits
+
+
 def group_entries(ids: torch.Tensor, k: int, n_expert: int, blobs_ptr: int, stride: int, bufs=None, stream=None):
     """Decode grouping (k_group): returns grp_ptr, grp_start, n_groups, ent_dst, ent_tok (device tensors)."""
     n_ent = ids.numel()
@@ -200,7 +299,7 @@ def route_sort(ids: torch.Tensor, k: int, n_expert: int, bufs=None, stream=None)
 
 
 def moe_combine(x, parts, wts, k: int, prow=None, shared=None, sgate=None, sg_stride: int = 1, stream=None) -> None:
-    """x[t] += sum_j w[t][j] parts[p(t,j)] (+ sigmoid(sgate[t]) shared[t]), in place."""
+    """x[t] += sum_j w[t][j] parts[p(t,j)] (+ sigmoid(sgate[t]) shared[t]), in place; a prow below 0 adds nothing."""
     n_tok, n = x.shape
     check(lib().tsx_moe_combine(_p(x), _p(parts), _p(prow), _p(wts), k, _p(shared), _p(sgate), sg_stride, n, n_tok,
                                 _stream(stream)), "moe_combine")
@@ -212,6 +311,33 @@ def moe_combine_norm(x, parts, wts, k: int, norm_w, eps: float, h, hq=None, prow
     n_tok, n = x.shape
     check(lib().tsx_moe_combine_norm(_p(x), _p(parts), _p(prow), _p(wts), k, _p(shared), _p(sgate), sg_stride, n, n_tok,
                                      _p(norm_w), eps, _p(h), _p(hq), _stream(stream)), "moe_combine_norm")
+
+
+def moe_combine_backward(dy, parts, wts, k: int, prow=None, shared=None, sgate=None, sg_stride: int = 1, dwts=None,
+                         dparts=None, dshared=None, dsgate=None, stream=None) -> None:
+    """The gradients of moe_combine from dy [n_tok, n], into those of dwts [n_tok, k], dparts (parts' shape), dshared
+    [n_tok, n] and dsgate [n_tok] that are given."""
+    what = "moe_combine_backward"
+    _expect(what, "dy", dy, (dy.shape[0], dy.shape[-1]), torch.float32)
+    n_tok, n = dy.shape
+    _expect(what, "parts", parts, (parts.shape[0], n), torch.float32, dy)
+    if prow is None and parts.shape[0] < n_tok * k:
+        raise ValueError(f"{what}: {parts.shape[0]} part rows for {n_tok} tokens x {k}")
+    _expect(what, "wts", wts, (n_tok, k), torch.float32, dy)
+    if prow is not None:
+        _expect(what, "prow", prow.view(-1), (n_tok * k,), torch.int32, dy)
+    _expect(what, "shared", shared, (n_tok, n), torch.float32, dy)
+    if sgate is not None:
+        left = sgate.untyped_storage().nbytes() // 4 - sgate.storage_offset()
+        if sgate.dtype != torch.float32 or sgate.device != dy.device or sg_stride < 0 or (
+                n_tok and left <= (n_tok - 1) * sg_stride):
+            raise ValueError(f"{what}: sgate in fp32 on {dy.device}, a value per token {sg_stride} apart")
+    _expect(what, "dwts", dwts, (n_tok, k), torch.float32, dy)
+    _expect(what, "dparts", dparts, parts.shape, torch.float32, dy)
+    _expect(what, "dshared", dshared, (n_tok, n), torch.float32, dy)
+    _expect(what, "dsgate", dsgate, (n_tok,), torch.float32, dy)
+    _launch(what, lib().tsx_moe_combine_backward, dy, stream, _p(dy), _p(parts), _p(prow), _p(wts), k, _p(shared),
+            _p(sgate), sg_stride, n, n_tok, _p(dwts), _p(dparts), _p(dshared), _p(dsgate))
 
 
 # ------------------------------------------------------------------ prefill

@@ -307,6 +307,38 @@ TSX_API int tsx_moe_mmq_gate_up_swiglu(const void* w, int type, int64_t n_ff, in
                                        int n_exp, const void* xq, int64_t x_rows, const int32_t* xids,
                                        const int32_t* bounds, int64_t n_rows, void* hq, void* stream);
 
+/* ------------------------------------------------------------------------------------------------ adapters */
+/* Low-rank adapters of many requests beside a projection that all rows share (an expert-independent one: the shared
+ * expert's gate, up or down product): adapter i is B_i A_i times scale[i], A_i [rank][n_in] at a + i * a_stride values and
+ * B_i [n_out][rank] at b + i * b_stride, both row-major of `type` (the layout of a GGUF adapter's lora_a and lora_b).  An
+ * adapter of a smaller rank is filled up with zeros.  rank 1..256. */
+typedef struct {
+    int32_t type; /* TSX_F32, TSX_F16 or TSX_BF16 */
+    int32_t n;    /* adapters, 0 or more */
+    int32_t rank, n_in, n_out;
+    const void* a;
+    const void* b;
+    int64_t a_stride, b_stride;
+    const float* scale; /* device [n], or null: 1 */
+} tsx_adapters;
+/* y[j] = base[j] + scale[a] * B_a (A_a x[j]) with a = ids[j], for `rows` rows of x (n_in floats, ld_x apart), base and y
+ * (n_out floats); an id outside [0, n) is a row without an adapter: y[j] = base[j].  base may be y (rows without an adapter
+ * are then not touched) or null (0).  The sums are in fp32.  One launch, no scratch; one token or many. */
+TSX_API int tsx_moe_adapters(const tsx_adapters* p, const int32_t* ids, const float* x, int64_t ld_x, const float* base,
+                             int64_t ld_base, float* y, int64_t ld_y, int64_t rows, void* stream);
+/* The gradients of tsx_moe_adapters from dy [rows][n_out]:
+ *   dx[j] = dbase[j] + A_a^T v_j with v_j = scale[a] * B_a^T dy[j]   (dbase: the gradient through the projection itself; it may
+ *           be dx, or null for 0; a row without an adapter has dx[j] = dbase[j])
+ *   da[i] = sum over the rows of adapter i of v_j x[j]^T  (fp32 [n][rank][n_in]),
+ *   db[i] = scale[i] * sum of dy[j] (A_i x[j])^T          (fp32 [n][n_out][rank]), both dense and written whole: 0 for an
+ *           adapter without rows.  The sums' order depends on the ids alone.
+ * Each of dx, da, db may be null.  n up to 512.  scratch: tsx_moe_adapters_scratch_bytes(p, rows) bytes, 256-byte aligned,
+ * nothing kept in it from one call for the next (calls that may overlap need one each). */
+TSX_API size_t tsx_moe_adapters_scratch_bytes(const tsx_adapters* p, int64_t rows);
+TSX_API int tsx_moe_adapters_backward(const tsx_adapters* p, const int32_t* ids, const float* x, int64_t ld_x,
+                                      const float* dy, int64_t ld_dy, const float* dbase, int64_t ld_dbase, float* dx,
+                                      int64_t ld_dx, float* da, float* db, int64_t rows, void* scratch, void* stream);
+
 /* ------------------------------------------------------------------------------------------------ checks and data */
 /* The integer contract: sums[(r*ncols + c)*nsub + u] = sum over sub-block u (32 values) of w_int * a_int, and
  * qsums (may be null) the same for sum a_int, for rows [0, n_rows) of W against ncols Q8_1 activations.  An expert

@@ -84,6 +84,13 @@ class RouterArgs(C.Structure):
                 ] + [("scale", C.c_float), ("floor", C.c_float), ("bias", C.c_void_p)]
 
 
+class AdapterArgs(C.Structure):
+    """tsx_adapters: low-rank adapters beside one projection."""
+
+    _fields_ = [(n, C.c_int32) for n in ("type", "n", "rank", "n_in", "n_out")] + [
+        ("a", C.c_void_p), ("b", C.c_void_p), ("a_stride", C.c_int64), ("b_stride", C.c_int64), ("scale", C.c_void_p)]
+
+
 class GgufTensor(C.Structure):
     """tsx_gguf_tensor: one entry of a GGUF tensor directory (reference TensorInfo)."""
 
@@ -196,6 +203,9 @@ SIGNATURES = {
     "tsx_moe_mmq_run": (I32, [C.POINTER(MmqProduct), P]),
     "tsx_moe_mmq_swiglu": (I32, [P, P, I64, I64, I32, P]),
     "tsx_moe_mmq_gate_up_swiglu": (I32, [P, I32, I64, I64, U64, I32, P, I64, P, P, I64, P, P]),
+    "tsx_moe_adapters": (I32, [C.POINTER(AdapterArgs), P, P, I64, P, I64, P, I64, I64, P]),
+    "tsx_moe_adapters_scratch_bytes": (SZ, [C.POINTER(AdapterArgs), I64]),
+    "tsx_moe_adapters_backward": (I32, [C.POINTER(AdapterArgs), P, P, I64, P, I64, P, I64, P, I64, P, P, I64, P, P]),
     "tsx_moe_subblock_sums": (I32, [I32, P, I64, I64, P, I64, P, P, P]),
     "tsx_moe_quantize_weights": (I32, [I32, P, I64, I64, P]),
 }

@@ -32,6 +32,7 @@ SOURCES = [
     "tsx_layer.hip",
     "tsx_route.hip",
     "tsx_router.hip",
+    "tsx_adapters.hip",
     "tsx_prefill.hip",
 ]
 

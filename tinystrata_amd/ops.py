@@ -11,8 +11,8 @@ import ctypes as C
 import numpy as np
 import torch
 
-from ._lib import (BF16, F16, F32, IQ3_S, IQ3_XXS, Q4_K, Q8_0, ExpertLayout, MmqProduct, MmvqIds, MmvqSlots, RouterArgs,
-                   check, lib)
+from ._lib import (BF16, F16, F32, IQ3_S, IQ3_XXS, Q4_K, Q8_0, AdapterArgs, ExpertLayout, MmqProduct, MmvqIds, MmvqSlots,
+                   RouterArgs, check, lib)
 
 WEIGHT_TYPES = (Q8_0, Q4_K, IQ3_XXS, IQ3_S)
 Q8_1_BLOCK_BYTES = 36
@@ -391,6 +391,70 @@ def mmq_gate_up_swiglu(w, ggml_type: int, n_ff: int, n_embd: int, expert_bytes: 
     check(lib().tsx_moe_mmq_gate_up_swiglu(_p(w), ggml_type, n_ff, n_embd, expert_bytes, n, _p(xq), x_rows, _p(xids),
                                             _p(bounds), n_rows, _p(hq), _stream(stream)), "mmq_gate_up_swiglu")
     return hq
+
+
+# ------------------------------------------------------------------ adapters
+class Adapters:
+    """Low-rank adapters beside one projection (tsx_adapters): a [n, rank, n_in] and b [n, n_out, rank] in fp32, fp16 or
+    bf16, each adapter's matrix dense; scale [n] fp32 or None (1).  Read at every call: they may be updated in place."""
+
+    def __init__(self, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor | None = None):
+        if a.dim() != 3 or b.dim() != 3 or a.dtype not in PLAIN_TYPES:
+            raise ValueError("Adapters: a [n, rank, n_in] and b [n, n_out, rank] in fp32, fp16 or bf16")
+        n, rank, n_in = a.shape
+        n_out = b.shape[1]
+        for name, t, rows, cols in (("a", a, rank, n_in), ("b", b, n_out, rank)):
+            if tuple(t.shape) != (n, rows, cols) or t.dtype != a.dtype or t.device != a.device:
+                raise ValueError(f"Adapters: {name} is {t.dtype} {tuple(t.shape)} on {t.device}, not {a.dtype} "
+                                 f"{(n, rows, cols)} on {a.device}")
+            if t.numel() and not t[0].is_contiguous():
+                raise ValueError(f"Adapters: {name}'s matrices are not dense (strides {t.stride()})")
+        _expect("Adapters", "scale", scale, (n,), torch.float32, a)
+        self.a, self.b, self.scale = a, b, scale
+        self.n, self.rank, self.n_in, self.n_out = n, rank, n_in, n_out
+        self.args = AdapterArgs(type=PLAIN_TYPES[a.dtype], n=n, rank=rank, n_in=n_in, n_out=n_out, a=a.data_ptr(),
+                                b=b.data_ptr(), a_stride=a.stride(0) if n > 1 else rank * n_in,
+                                b_stride=b.stride(0) if n > 1 else rank * n_out,
+                                scale=None if scale is None else scale.data_ptr())
+
+
+def adapters(ad: Adapters, ids: torch.Tensor, x: torch.Tensor, y: torch.Tensor, base: torch.Tensor | None = None,
+             stream=None) -> torch.Tensor:
+    """y[j] = base[j] + scale B (A x[j]) with the adapter ids[j] (int32; outside [0, n): none), rows of x [rows, n_in],
+    base and y [rows, n_out] possibly apart; base may be y, or None for 0."""
+    rows = ids.shape[0]
+    _expect("adapters", "ids", ids, (rows,), torch.int32, x)
+    _expect("adapters", "x", x, (rows, ad.n_in), torch.float32, ad.a, rows=True)
+    _expect("adapters", "y", y, (rows, ad.n_out), torch.float32, x, rows=True)
+    _expect("adapters", "base", base, (rows, ad.n_out), torch.float32, x, rows=True)
+    _launch("adapters", lib().tsx_moe_adapters, x, stream, C.byref(ad.args), _p(ids), _p(x), _ld(x), _p(base), _ld(base),
+            _p(y), _ld(y), rows)
+    return y
+
+
+def adapters_scratch_bytes(ad: Adapters, rows: int) -> int:
+    return lib().tsx_moe_adapters_scratch_bytes(C.byref(ad.args), rows)
+
+
+def adapters_backward(ad: Adapters, ids: torch.Tensor, x: torch.Tensor, dy: torch.Tensor, dx=None, da=None, db=None,
+                      dbase=None, scratch=None, stream=None) -> None:
+    """The gradients of adapters() from dy [rows, n_out], into those of dx [rows, n_in] (= dbase + ..), da [n, rank, n_in]
+    and db [n, n_out, rank] (fp32) that are given."""
+    what, rows = "adapters_backward", ids.shape[0]
+    _expect(what, "ids", ids, (rows,), torch.int32, x)
+    _expect(what, "x", x, (rows, ad.n_in), torch.float32, ad.a, rows=True)
+    _expect(what, "dy", dy, (rows, ad.n_out), torch.float32, x, rows=True)
+    _expect(what, "dx", dx, (rows, ad.n_in), torch.float32, x, rows=True)
+    _expect(what, "dbase", dbase, (rows, ad.n_in), torch.float32, x, rows=True)
+    _expect(what, "da", da, ad.a.shape, torch.float32, x)
+    _expect(what, "db", db, ad.b.shape, torch.float32, x)
+    need = adapters_scratch_bytes(ad, rows)
+    if scratch is None:
+        scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
+    elif scratch.device != x.device or not scratch.is_contiguous() or scratch.numel() * scratch.element_size() < need:
+        raise ValueError(f"{what}: scratch of {need} bytes on {x.device} (adapters_scratch_bytes)")
+    _launch(what, lib().tsx_moe_adapters_backward, x, stream, C.byref(ad.args), _p(ids), _p(x), _ld(x), _p(dy), _ld(dy),
+            _p(dbase), _ld(dbase), _p(dx), _ld(dx), _p(da), _p(db), rows, _p(scratch))
 
 
 # ------------------------------------------------------------------ checks and data

@@ -35,8 +35,8 @@ struct RouteArgs {
     int32_t* prow;
     int32_t* counts;
     float scale, floor;
-    int type, sigmoid, norm, vec, need64;
-    int n_tok, n_expert, k, n_group, topk_group, group_top, group_size, lg_shift;
+    int type, sigmoid, norm, vec, vec_bias, need64;
+    int n_tok, n_expert, k, n_group, topk_group, group_top, group_size, shift;
 };
 
 // logit e of a row, and four of them from e on (row + e aligned to four elements)
@@ -85,14 +85,17 @@ __device__ __forceinline__ double rcp64(double d) {
     return __builtin_fma(__builtin_fma(-d, y, 1.0), y, y);
 }
 
-// c with the low bits of its mantissa replaced so that among equal c the lower id is the larger key
+// c with the low bits of its mantissa replaced so that among equal c the lower id is the larger key.  c = -inf stands for
+// none: its key lies below kNone, and every other one above (a c that fp32 values make is far from the ends of the range).
+constexpr double kNone = -1e308;
 template <int BITS>
 __device__ __forceinline__ double pack_key(double c, uint32_t id) {
-    constexpr uint64_t mask = (1ull << BITS) - 1;
-    c = __builtin_fmin(c, 1.79769313486231e308) + 0.0;  // +inf would become a NaN; -0 and 0 are equal
+    constexpr uint32_t mask = (1u << BITS) - 1;
+    // an infinity would become a NaN; -0 and 0 are equal
+    c = __builtin_fmax(__builtin_fmin(c, 1.79769313486231e308), -1.79769313486231e308) + 0.0;
     const uint64_t u = __builtin_bit_cast(uint64_t, c);
-    const uint64_t low = (u >> 63) ? id : mask - id;
-    return __builtin_bit_cast(double, (u & ~mask) | low);
+    const uint32_t low = (mask - id) ^ ((uint32_t) ((int32_t) (u >> 32) >> 31) & mask);
+    return __builtin_bit_cast(double, (u & ~(uint64_t) mask) | low);
 }
 template <int BITS>
 __device__ __forceinline__ int key_id(double key) {
@@ -132,6 +135,12 @@ __device__ __forceinline__ float token_reduce(float v, Op op) {
 template <int L, int M = 1>
 __device__ __forceinline__ double token_sum(double v) {
     if constexpr (M < L) return token_sum<L, 2 * M>(v + swap64<M>(v));
+    return v;
+}
+
+template <int L, int M = 1>
+__device__ __forceinline__ double token_min(double v) {
+    if constexpr (M < L) return token_min<L, 2 * M>(__builtin_fmin(v, swap64<M>(v)));
     return v;
 }
 
@@ -187,153 +196,328 @@ __device__ __forceinline__ void merge_two(double& m1, double& m2, int lanes) {
     }
 }
 
-// A token's L lanes, L >> lg_shift.. : lane = group * Lg + i with Lg = 1 << lg_shift lanes per group (one group: Lg = L);
-// the lane holds the four experts from 4 (i + Lg q) of its group on, q < V / 4.
-template <int L, int V, int K>
-__global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
+// How a token's experts lie on L lanes: lane = group * lanes + i with `lanes` = 1 << shift of them per group (one group: all
+// L); the lane holds the four experts from 4 (i + lanes q) of its group on, q < V / 4.
+struct Place {
+    int i, lanes, size, e0;
+    __device__ __forceinline__ Place(const RouteArgs& a, int sub, int shift) {
+        const int g = sub >> shift;
+        lanes = 1 << shift;
+        i = sub & (lanes - 1);
+        size = g < a.n_group ? a.group_size : 0;
+        e0 = g * a.group_size;
+    }
+    __device__ __forceinline__ int pos(int v) const { return 4 * (i + lanes * (v / 4)) + v % 4; }
+};
+// the lane's logits (-inf for one that takes no part), and biases
+template <int V>
+__device__ __forceinline__ void fetch_logits(const RouteArgs& a, const void* row, const Place& p, float (&l)[V]) {
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q) {
+        const int pos = p.pos(4 * q);
+        float o[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (a.vec) {
+            if (pos < p.size) logits4_at(row, a.type, p.e0 + pos, o);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (pos + c < p.size) o[c] = logit_at(row, a.type, p.e0 + pos + c);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) l[4 * q + c] = live_logit(o[c]);
+    }
+}
+template <int V>
+__device__ __forceinline__ void fetch_bias(const RouteArgs& a, const Place& p, float (&b)[V]) {
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q) {
+        const int pos = p.pos(4 * q);
+        float4 o = {0.f, 0.f, 0.f, 0.f};
+        if (a.vec_bias) {
+            if (pos < p.size) o = *(const float4*) (a.bias + p.e0 + pos);
+        } else {
+            if (pos < p.size) o.x = a.bias[p.e0 + pos];
+            if (pos + 1 < p.size) o.y = a.bias[p.e0 + pos + 1];
+            if (pos + 2 < p.size) o.z = a.bias[p.e0 + pos + 2];
+            if (pos + 3 < p.size) o.w = a.bias[p.e0 + pos + 3];
+        }
+        b[4 * q] = o.x, b[4 * q + 1] = o.y, b[4 * q + 2] = o.z, b[4 * q + 3] = o.w;
+    }
+}
+// a group's value on every lane of it, with the group's number in its low bits, and how many groups come before it
+template <int L, int V>
+__device__ __forceinline__ double group_rank(const RouteArgs& a, const double (&key)[V], int sub, int shift, int& before) {
+    double m1 = -INFINITY, m2 = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        m2 = __builtin_fmax(m2, __builtin_fmin(m1, key[v]));
+        m1 = __builtin_fmax(m1, key[v]);
+    }
+    merge_two<L>(m1, m2, 1 << shift);
+    if (a.group_top == 2 && m2 > -INFINITY) m1 += m2;
+    const double mine = pack_key<kGroupBits>(m1, (uint32_t) (sub >> shift) & 63u);
+    before = 0;
+    for (int o = 0; o < a.n_group; ++o) before += __shfl(mine, o << shift, L) > mine;
+    return mine;
+}
+
+// the wave's largest value, in every lane: within the rows of 16 by exchanges, then the four rows' read out
+__device__ __forceinline__ double wave_max64(double v) {
+    v = -token_min<16>(-v);
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    auto row = [&](int l) {
+        const uint32_t lo = (uint32_t) __builtin_amdgcn_readlane((int) (uint32_t) u, l);
+        const uint32_t hi = (uint32_t) __builtin_amdgcn_readlane((int) (uint32_t) (u >> 32), l);
+        return __builtin_bit_cast(double, (uint64_t) hi << 32 | lo);
+    };
+    return __builtin_fmax(__builtin_fmax(row(0), row(16)), __builtin_fmax(row(32), row(48)));
+}
+
+// One token's picks in 64 bits by a whole wave: lane r returns pick r, -1 for none.  Expert e = lane + 64 i; `keys` are
+// kMaxExperts values of LDS, the wave's own, for the sums over groups.  The rare way (every wave of a batch waits for the one
+// that takes it, so its latency counts: 4 us): k rounds of the largest key below the last one.
+__device__ __forceinline__ int pick_precise(const RouteArgs& a, const void* row, int lane, double* keys) {
+    constexpr int V = kMaxExperts / 64;
+    const int E = a.n_expert;
+    float l[V];
+    float m = a.sigmoid ? 0.f : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < V; ++i) l[i] = lane + 64 * i < E ? live_logit(logit_at(row, a.type, lane + 64 * i)) : -INFINITY;
+    if (!a.sigmoid) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) m = __builtin_fmaxf(m, l[i]);
+        m = token_reduce<64>(m, OpMax());
+    }
+    const bool any = m > -INFINITY && m < INFINITY;
+    double key[V], total = 0.0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        key[i] = -1.0;  // takes no part
+        if (64 * i < E) {
+            double s = exp64(a.sigmoid ? -(double) l[i] : (double) l[i] - (double) m);
+            if (a.sigmoid) s = rcp64(1.0 + s);
+            if (any && l[i] > -INFINITY) {
+                key[i] = s;
+                total += s;
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);  // one after the other: side by side they would take the register file
+    }
+    const double r = a.sigmoid ? 1.0 : 1.0 / token_sum<64>(total);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int e = lane + 64 * i;
+        const double c = __builtin_fma(key[i], r, a.bias && e < E ? (double) a.bias[e] : 0.0);
+        key[i] = key[i] >= 0.0 && c > -INFINITY ? c : -INFINITY;  // (a bias may be NaN)
+    }
+    uint64_t kept = ~0ull;
+    if (a.n_group > 1) {  // lane g: group g
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (lane + 64 * i < E) keys[lane + 64 * i] = key[i];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        double m1 = -INFINITY, m2 = -INFINITY;
+        const int e0 = min(lane, a.n_group - 1) * a.group_size;
+#pragma unroll 4
+        for (int j = 0; j < a.group_size; ++j) {
+            const double c = keys[e0 + j];
+            m2 = __builtin_fmax(m2, __builtin_fmin(m1, c));
+            m1 = __builtin_fmax(m1, c);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (a.group_top == 2 && m2 > -INFINITY) m1 += m2;
+        const double mine = pack_key<kGroupBits>(m1, (uint32_t) lane);
+        int before = 0;
+        for (int o = 0; o < a.n_group; ++o) before += __shfl(mine, o, 64) > mine;
+        kept = __ballot(lane < a.n_group && before < a.topk_group);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int e = lane + 64 * i;
+        double c = key[i];
+        if (a.n_group > 1 && !(kept >> (e / a.group_size) & 1)) c = -INFINITY;
+        if (!a.bias && c > -INFINITY) c = (double) l[i];  // the experts' own order is that of the logits
+        key[i] = pack_key<kIdBits>(c, (uint32_t) e);
+    }
+    double last = INFINITY;
+    int id = -1;
+    for (int j = 0; j < a.k; ++j) {
+        double best = -INFINITY;  // nothing below the last one
+#pragma unroll
+        for (int i = 0; i < V; ++i) best = key[i] < last ? __builtin_fmax(best, key[i]) : best;
+        last = wave_max64(best);
+        if (lane == j && last > kNone) id = key_id<kIdBits>(last);
+    }
+    return id;
+}
+
+// Choice values that need the scores are formed in fp32, from the hardware's exponential and reciprocal, and the selection is
+// made on them; only where two values that decide it lie within those roundings of each other is it made again in 64 bits.
+// `slack` bounds how far a value in fp32 is from the exact one.  A sigmoid: the exponential is off by 1.5 |l| + 2 units of
+// 2^-24, which s (1 - s) takes to less than 1, the sum with 1 and the reciprocal by 3; the sum with the bias by half a step of
+// at most 1 + |bias|: 5 + |bias| units in all.  A softmax: (2.5 |l - m| + 30) units of its size, |l - m| below 104 where it is
+// not 0, and half a step for the sum: less than 2^-15 of |c| + |bias|.  Equal logits with equal biases have equal values in
+// any precision and need no second look.
+//
+// Measured (us, sigmoid scores, bias, 8 groups by their two largest, top-8 of 256): 16384 tokens in 64 bits throughout 35.
+// Sixteen lanes a token or 64: one token 7.3 or 5.0, 2048 (no groups) 4.5 or 4.3, 4096 4.5 or 5.7, 16384 7.6 or 15.1; of 64
+// experts 2.6 or 3.4 at one token already.
+template <int L, int V, int K, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) route_kernel(RouteArgs a) {
     extern __shared__ int s_count[];
+    __shared__ double s_keys[WAVES][kMaxExperts];
     const int lane = threadIdx.x & 63, sub = lane & (L - 1);
     if (a.counts) {
-        for (int e = threadIdx.x; e < a.n_expert; e += 256) s_count[e] = 0;
+        for (int e = threadIdx.x; e < a.n_expert; e += 64 * WAVES) s_count[e] = 0;
         __syncthreads();
     }
-    const int per_block = 4 * (64 / L);
+    constexpr int per_block = WAVES * (64 / L);
+    const Place p(a, sub, a.shift);
     // every lane stays for the exchanges; a group of lanes past the last token repeats it and stores nothing
-    for (int t0 = blockIdx.x * per_block; t0 < a.n_tok; t0 += gridDim.x * per_block) {
-        const int tt = t0 + (int) threadIdx.x / L, t = min(tt, a.n_tok - 1);
-        const int g = sub >> a.lg_shift, lg = 1 << a.lg_shift, i = sub & (lg - 1);
-        const int size = g < a.n_group ? a.group_size : 0, e0 = g * a.group_size;
-        const void* row = (const char*) a.logits + (int64_t) t * a.ld * (a.type == TSX_F32 ? 4 : 2);
-        float l[V];
+    const int64_t t0 = (int64_t) blockIdx.x * per_block;
+    const int64_t tt = t0 + (int) threadIdx.x / L, t = tt < a.n_tok ? tt : a.n_tok - 1;
+    const void* row = (const char*) a.logits + t * a.ld * (a.type == TSX_F32 ? 4 : 2);
+    float c[V];  // the choice values
+    fetch_logits<V>(a, row, p, c);
+    float m = 0.f, sum = 1.f, most_bias = 0.f;
+    constexpr float kLog2e = 1.44269504f;
+    if (!a.sigmoid) {
+        m = -INFINITY;
 #pragma unroll
-        for (int q = 0; q < V / 4; ++q) {
-            const int pos = 4 * (i + lg * q);
-            float o[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            if (a.vec) {
-                if (pos < size) logits4_at(row, a.type, e0 + pos, o);
-            } else {
+        for (int v = 0; v < V; ++v) m = __builtin_fmaxf(m, c[v]);
+        m = token_reduce<L>(m, OpMax());
+        sum = 0.f;
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (pos + c < size) o[c] = logit_at(row, a.type, e0 + pos + c);
-            }
-#pragma unroll
-            for (int c = 0; c < 4; ++c) l[4 * q + c] = live_logit(o[c]);
-        }
-        float m = 0.f, sum = 1.f;
-        if (!a.sigmoid) {
-            m = -INFINITY;
-#pragma unroll
-            for (int v = 0; v < V; ++v) m = __builtin_fmaxf(m, l[v]);
-            m = token_reduce<L>(m, OpMax());
-        }
-        // a softmax over a logit of +inf has no values, and one over nothing none either
-        const bool any = a.sigmoid || (m > -INFINITY && m < INFINITY);
-        double key[V];
-        if (a.need64) {
-            double c[V];
-            double total = 0.0;
-            if (a.sigmoid) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) c[v] = rcp64(1.0 + exp64(-(double) l[v]));
-            } else {
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    c[v] = l[v] > -INFINITY ? exp64((double) l[v] - (double) m) : 0.0;
-                    total += c[v];
-                }
-                total = token_sum<L>(total);
-                sum = (float) total;
-                const double r = any ? 1.0 / total : 0.0;
-#pragma unroll
-                for (int v = 0; v < V; ++v) c[v] *= r;
-            }
-            if (a.bias) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const int pos = 4 * (i + lg * (v / 4)) + v % 4;
-                    if (pos < size) c[v] += (double) a.bias[e0 + pos];
-                }
-            }
-#pragma unroll
-            for (int v = 0; v < V; ++v) key[v] = any && l[v] > -INFINITY && c[v] > -INFINITY ? c[v] : -INFINITY;
-        } else {
-            if (!a.sigmoid) {
-                sum = 0.f;
-#pragma unroll
-                for (int v = 0; v < V; ++v) sum += expf(l[v] - m);  // -inf and no other: NaN, unused
-                sum = token_reduce<L>(sum, OpAdd());
-            }
-#pragma unroll
-            for (int v = 0; v < V; ++v) key[v] = any ? (double) l[v] : -INFINITY;
-        }
-        if (a.n_group > 1) {
-            double m1 = -INFINITY, m2 = -INFINITY;
-            // without a bias the largest logit has the largest score; sums need the scores, and need64 brought them
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                m2 = __builtin_fmax(m2, __builtin_fmin(m1, key[v]));
-                m1 = __builtin_fmax(m1, key[v]);
-            }
-            merge_two<L>(m1, m2, lg);
-            double gv = m1;
-            if (a.group_top == 2 && m2 > -INFINITY) gv += m2;
-            const double mine = gv > -INFINITY ? pack_key<kGroupBits>(gv, (uint32_t) g & 63u) : -INFINITY;
-            int better = 0;  // groups before this one
-            for (int o = 0; o < a.n_group; ++o) better += __shfl(mine, o << a.lg_shift, L) > mine;
-            if (better >= a.topk_group) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) key[v] = -INFINITY;
-            }
-            if (a.need64 && !a.bias) {  // the experts' own order without a bias is that of the logits
-#pragma unroll
-                for (int v = 0; v < V; ++v) key[v] = key[v] > -INFINITY ? (double) l[v] : -INFINITY;
-            }
-        }
+        for (int v = 0; v < V; ++v) sum += __builtin_amdgcn_exp2f((c[v] - m) * kLog2e);  // (of -inf: 0)
+        sum = token_reduce<L>(sum, OpAdd());
+    }
+    // a softmax over a logit of +inf has no values, and one over nothing none either
+    const bool any = a.sigmoid || (m > -INFINITY && m < INFINITY);
+    if (a.need64) {
+        float b[V] = {};
+        if (a.bias) fetch_bias<V>(a, p, b);
+        const float r = __builtin_amdgcn_rcpf(sum);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const int e = e0 + 4 * (i + lg * (v / 4)) + v % 4;
-            key[v] = key[v] > -INFINITY ? pack_key<kIdBits>(key[v], (uint32_t) e) : -INFINITY;
+            const float s = a.sigmoid ? __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-c[v] * kLog2e))
+                                      : __builtin_amdgcn_exp2f((c[v] - m) * kLog2e) * r;
+            const float sb = s + b[v];
+            c[v] = any && c[v] > -INFINITY && sb > -INFINITY ? sb : -INFINITY;
+            if (fabsf(b[v]) < INFINITY) most_bias = __builtin_fmaxf(most_bias, fabsf(b[v]));
         }
-        double top[K];
-        if constexpr (V <= K) {
-            sort_keys<V>(key);
+        most_bias = token_reduce<L>(most_bias, OpMax());
+    } else {
 #pragma unroll
-            for (int v = 0; v < K; ++v) top[v] = v < V ? key[v < V ? v : 0] : -INFINITY;
-        } else {
-            static_assert(V == 2 * K, "a lane's keys sort as one list or two");
-            sort_keys<K>(key);
-            sort_keys<K>(key + K);
-            double second[K];
+        for (int v = 0; v < V; ++v) c[v] = any ? c[v] : -INFINITY;
+    }
+    auto slack = [&](double x) -> double {
+        return a.sigmoid ? (6.0 + (double) most_bias) * 0x1p-24 : (__builtin_fabs(x) + (double) most_bias) * 0x1p-15;
+    };
+    bool open = false, kept = true;  // open: the values in fp32 do not decide
+    double key[V];
 #pragma unroll
-            for (int v = 0; v < K; ++v) top[v] = key[v], second[v] = key[K + v];
-            merge_top<K>(top, second);
-        }
-        merge_lanes<L, K>(top);
-        // lane j of the token takes pick j
-        double mine = top[0];
+    for (int v = 0; v < V; ++v) key[v] = (double) c[v];
+    if (a.n_group > 1) {
+        int before;
+        const double mine = group_rank<L, V>(a, key, sub, a.shift, before);
+        kept = before < a.topk_group;
+        if (a.need64) {  // the least group kept and the best one dropped
+            const double least = token_min<L>(kept ? mine : (double) INFINITY);
+            const double best = -token_min<L>(kept ? (double) INFINITY : -mine);
+            open = best > kNone && least - best <= 2.0 * (slack(least) + slack(best));
+            if (!a.bias) {  // the experts' own order without a bias is that of the logits
+                float l[V];
+                fetch_logits<V>(a, row, p, l);
 #pragma unroll
-        for (int j = 1; j < K; ++j) mine = sub == j ? top[j] : mine;
-        const bool picked = sub < a.k && mine > -INFINITY;
-        const int id = picked ? key_id<kIdBits>(mine) : -1;
-        float s = 0.f;
-        if (picked) {
-            const float lj = logit_at(row, a.type, id);
-            s = a.sigmoid ? 1.0f / (1.0f + expf(-lj)) : expf(lj - m) / sum;
+                for (int v = 0; v < V; ++v) key[v] = c[v] > -INFINITY ? (double) l[v] : -INFINITY;
+            }
         }
-        float w = s * a.scale;
-        if (a.norm) w *= 1.0f / __builtin_fmaxf(token_reduce<L>(s, OpAdd()), a.floor);
-        if (tt < a.n_tok && sub < a.k) {
-            const int64_t ent = (int64_t) tt * a.k + sub;
-            a.ids[ent] = id;
-            a.wts[ent] = w;
-            if (a.prow) a.prow[ent] = id < 0 ? -1 : (int32_t) ent;
-            if (a.counts && id >= 0) atomicAdd(&s_count[id], 1);
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) key[v] = pack_key<kIdBits>(kept ? key[v] : -INFINITY, (uint32_t) (p.e0 + p.pos(v)));
+    double top[K];
+    if constexpr (V <= K) {
+        sort_keys<V>(key);
+#pragma unroll
+        for (int v = 0; v < K; ++v) top[v] = v < V ? key[v < V ? v : 0] : -INFINITY;
+    } else {
+        static_assert(V == 2 * K, "a lane's keys sort as one list or two");
+        sort_keys<K>(key);
+        sort_keys<K>(key + K);
+        double second[K];
+#pragma unroll
+        for (int v = 0; v < K; ++v) top[v] = key[v], second[v] = key[K + v];
+        merge_top<K>(top, second);
+    }
+    merge_lanes<L, K>(top);
+    // lane j of the token takes pick j
+    double mine = top[0], next = -INFINITY, last = top[0];
+#pragma unroll
+    for (int j = 1; j < K; ++j) {
+        mine = sub == j ? top[j] : mine;
+        next = sub == j - 1 ? top[j] : next;
+        last = j == a.k - 1 ? top[j] : last;
+    }
+    bool picked = sub < a.k && mine > kNone;
+    int id = picked ? key_id<kIdBits>(mine) : -1;
+    if (a.bias) {
+        // the order of neighbours among the picks, and the last pick against what is left
+        bool near = sub + 1 < a.k && next > kNone && mine - next <= 2.0 * slack(mine);
+        const float cl = (float) last, edge = cl - 2.f * (float) slack(last);  // the id's bits round away
+        const int el = key_id<kIdBits>(last);
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            near |= kept && last > kNone && c[v] >= edge && (c[v] < cl || (c[v] == cl && p.e0 + p.pos(v) > el));
+        if (__any(near)) {
+            if (sub + 1 < a.k && next > kNone && mine - next <= 2.0 * slack(mine)) {
+                const int e = key_id<kIdBits>(next);
+                open |= !(logit_at(row, a.type, id) == logit_at(row, a.type, e) && a.bias[id] == a.bias[e]);
+            }
+            if (kept && last > kNone) {
+                const float ll = logit_at(row, a.type, el), bl = a.bias[el];
+                float l[V], b[V];
+                fetch_logits<V>(a, row, p, l);
+                fetch_bias<V>(a, p, b);
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+                    open |= c[v] >= edge && (c[v] < cl || (c[v] == cl && p.e0 + p.pos(v) > el)) &&
+                            !(l[v] == ll && b[v] == bl);
+            }
         }
+    }
+    if (const uint64_t again = __ballot(open)) {
+#pragma unroll 1
+        for (int o = 0; o < 64; o += L) {  // the wave's tokens with an open choice, one at a time
+            if (((again >> o) & (L == 64 ? ~0ull : (1ull << (L & 63)) - 1)) == 0) continue;
+            const int64_t to = t0 + (int) (threadIdx.x & ~63u) / L + o / L;
+            const void* r = (const char*) a.logits + (to < a.n_tok ? to : a.n_tok - 1) * a.ld * (a.type == TSX_F32 ? 4 : 2);
+            int own = lane;
+            asm volatile("" : "+v"(own));  // nothing of it is computed ahead of the loop, in registers of every wave
+            const int got = __shfl(pick_precise(a, r, own, s_keys[threadIdx.x >> 6]), sub, 64);
+            if ((lane & ~(L - 1)) == o) {
+                id = sub < a.k ? got : -1;
+                picked = id >= 0;
+            }
+        }
+    }
+    float s = 0.f;
+    if (picked) {
+        const float lj = logit_at(row, a.type, id);
+        s = a.sigmoid ? 1.0f / (1.0f + expf(-lj)) : expf(lj - m) / sum;
+    }
+    float w = s * a.scale;
+    if (a.norm) w *= 1.0f / __builtin_fmaxf(token_reduce<L>(s, OpAdd()), a.floor);
+    if (tt < a.n_tok && sub < a.k) {
+        const int64_t ent = tt * a.k + sub;
+        a.ids[ent] = id;
+        a.wts[ent] = w;
+        if (a.prow) a.prow[ent] = id < 0 ? -1 : (int32_t) ent;
+        if (a.counts && id >= 0) atomicAdd(&s_count[id], 1);
     }
     if (a.counts) {
         __syncthreads();
-        for (int e = threadIdx.x; e < a.n_expert; e += 256)
-            if (const int c = s_count[e]) atomicAdd(&a.counts[e], c);  // whole numbers: any order gives the same
+        for (int e = threadIdx.x; e < a.n_expert; e += 64 * WAVES)
+            if (const int n = s_count[e]) atomicAdd(&a.counts[e], n);  // whole numbers: any order gives the same
     }
 }
 
@@ -564,18 +748,17 @@ inline int pow2_at_least(int v) {
     return p;
 }
 
+template <int L, int V, int K, int WAVES>
+void launch_waves(const RouteArgs& a, hipStream_t st) {
+    constexpr int per_block = WAVES * (64 / L);
+    const unsigned blocks = (unsigned) (((int64_t) a.n_tok + per_block - 1) / per_block);
+    route_kernel<L, V, K, WAVES><<<blocks, 64 * WAVES, a.counts ? (size_t) a.n_expert * 4 : 0, st>>>(a);
+}
 template <int L, int V>
 void launch_route(const RouteArgs& a, hipStream_t st) {
-    const int per_block = 4 * (64 / L);
-    unsigned blocks = (unsigned) ((a.n_tok + per_block - 1) / per_block);
-    size_t lds = 0;
-    if (a.counts) {
-        // a block adds its counts once per expert at its end: no more blocks than fill the card
-        blocks = std::min(blocks, 1024u);
-        lds = (size_t) a.n_expert * 4;
-    }
-    if (a.k <= 8) route_kernel<L, V, 8><<<blocks, 256, lds, st>>>(a);
-    else route_kernel<L, V, 16><<<blocks, 256, lds, st>>>(a);
+    // with counts a block adds its own once per expert at its end: large blocks make these additions few
+    if (a.k <= 8) a.counts ? launch_waves<L, V, 8, 8>(a, st) : launch_waves<L, V, 8, 4>(a, st);
+    else a.counts ? launch_waves<L, V, 16, 8>(a, st) : launch_waves<L, V, 16, 4>(a, st);
 }
 
 }  // namespace
@@ -601,12 +784,14 @@ TSX_API int tsx_moe_route(const tsx_router* r, const void* logits, int64_t ld, i
     a.n_tok = n_tok, a.n_expert = r->n_expert, a.k = r->k, a.n_group = r->n_group, a.topk_group = r->topk_group;
     a.group_top = r->group_top, a.group_size = r->n_expert / r->n_group;
     a.need64 = r->bias != nullptr || (r->n_group > 1 && r->group_top == 2);
+    a.vec_bias = a.group_size % 4 == 0 && aligned(r->bias, 16);
     a.vec = a.group_size % 4 == 0 && ld % 4 == 0 && aligned(logits, 4 * elem_size(r->type));
-    // 16 lanes per token where each then holds at most 16 experts (four tokens share a wave's instructions), else 64
+    // 16 lanes per token where each then holds at most 16 experts (four tokens share a wave's instructions), but 64 while the
+    // tokens leave the card room and a lane of 16 would hold more than 8 (the shorter chains are then what counts)
     const int gp = pow2_at_least(r->n_group), quads = (a.group_size + 3) / 4;
     auto quads_per_lane = [&](int L) { return gp <= L ? (quads + L / gp - 1) / (L / gp) : 1 << 20; };
-    const int L = quads_per_lane(16) <= 4 ? 16 : 64, q = quads_per_lane(L);
-    for (int lanes = L / gp; lanes > 1; lanes /= 2) ++a.lg_shift;
+    const int q16 = quads_per_lane(16), L = q16 <= (n_tok <= 2048 ? 2 : 4) ? 16 : 64, q = quads_per_lane(L);
+    for (int lanes = L / gp; lanes > 1; lanes /= 2) ++a.shift;
     const hipStream_t st = (hipStream_t) stream;
     if (L == 16) {
         if (q <= 1) launch_route<16, 4>(a, st);

@@ -314,7 +314,7 @@ TSX_API int tsx_moe_mmq_gate_up_swiglu(const void* w, int type, int64_t n_ff, in
  * adapter of a smaller rank is filled up with zeros.  rank 1..256. */
 typedef struct {
     int32_t type; /* TSX_F32, TSX_F16 or TSX_BF16 */
-    int32_t n;    /* adapters, 0 or more */
+    int32_t n;    /* adapters, 0..4096 */
     int32_t rank, n_in, n_out;
     const void* a;
     const void* b;
@@ -332,7 +332,7 @@ TSX_API int tsx_moe_adapters(const tsx_adapters* p, const int32_t* ids, const fl
  *   da[i] = sum over the rows of adapter i of v_j x[j]^T  (fp32 [n][rank][n_in]),
  *   db[i] = scale[i] * sum of dy[j] (A_i x[j])^T          (fp32 [n][n_out][rank]), both dense and written whole: 0 for an
  *           adapter without rows.  The sums' order depends on the ids alone.
- * Each of dx, da, db may be null.  n up to 512.  scratch: tsx_moe_adapters_scratch_bytes(p, rows) bytes, 256-byte aligned,
+ * Each of dx, da, db may be null.  scratch: tsx_moe_adapters_scratch_bytes(p, rows) bytes, 256-byte aligned,
  * nothing kept in it from one call for the next (calls that may overlap need one each). */
 TSX_API size_t tsx_moe_adapters_scratch_bytes(const tsx_adapters* p, int64_t rows);
 TSX_API int tsx_moe_adapters_backward(const tsx_adapters* p, const int32_t* ids, const float* x, int64_t ld_x,

@@ -18,7 +18,7 @@ BACKWARD = [256, 256, 64, 256, 32, 256, 64, 1024, 64, 256, 256, 3, 256, None]
 
 
 @pytest.mark.parametrize("kw,rc", [(dict(type=_lib.Q8_0), -1), (dict(rank=0), -1), (dict(rank=257), -1), (dict(n_in=0), -1),
-                                   (dict(n_out=0), -1), (dict(n_in=(1 << 24) + 1), -1), (dict(n=-1), -2), (dict(a=None), -2),
+                                   (dict(n_out=0), -1), (dict(n_in=(1 << 24) + 1), -1), (dict(n=4097), -1), (dict(n=-1), -2), (dict(a=None), -2),
                                    (dict(b=None), -2), (dict(a=257), -2), (dict(b=257), -2), (dict(a_stride=1023), -2),
                                    (dict(b_stride=511), -2), (dict(scale=258), -2), (dict(type=_lib.F32, a=258), -2)])
 def test_adapters_refused(kw, rc):
@@ -47,8 +47,6 @@ def test_adapters_buffers_refused():
         b = list(BACKWARD)
         b[i] = v
         assert lib.tsx_moe_adapters_backward(C.byref(a), *b) == _lib.TSX_ERR_ARG, (i, v)
-    many = args(n=513)
-    assert lib.tsx_moe_adapters_backward(C.byref(many), *BACKWARD) == _lib.TSX_ERR_UNSUPPORTED
 
 
 def test_scratch_bytes():
@@ -56,7 +54,7 @@ def test_scratch_bytes():
     up = lambda v: (v + 255) // 256 * 256
     for rows, rank, pad in [(0, 16, 16), (5, 3, 16), (100, 33, 64), (4096, 100, 128), (7, 200, 256)]:
         a = args(rank=rank)
-        need = up(5 * 4) + up(4) + 3 * up(rows * 4) + 2 * up(rows * pad * 4)
+        need = 2 * up(rows * pad * 4)
         assert lib.tsx_moe_adapters_scratch_bytes(C.byref(a), rows) == need
     assert lib.tsx_moe_adapters_scratch_bytes(None, 5) == 0
     assert lib.tsx_moe_adapters_scratch_bytes(C.byref(args()), -1) == 0

@@ -120,6 +120,15 @@ def test_adapters_many_rows():
     check(c)
 
 
+@pytest.mark.parametrize("n,rows", [(4096, 70), (700, 5000), (300, 40), (2, 4097), (1, 4113)])
+def test_adapters_regrouped(n, rows):
+    """Mixed rows with many adapters, over the edges of the chunks that rows are regrouped in; a last chunk of one row."""
+    check(make(n, 4, 16, 20, rows, "some", torch.bfloat16, seed=rows, scaled=n != 300))
+    c = make(n, 4, 16, 20, rows, "segments", torch.float16, seed=n)
+    c["ids"][rows // 2:] = c["ids"][rows // 2:].flip(0)
+    check(c)
+
+
 def test_no_rows_and_no_adapters():
     c = make(2, 8, 32, 16, 0, "some", torch.float32)
     ad = ops.Adapters(c["a"], c["b"], c["scale"])

@@ -33,6 +33,7 @@ SOURCES = [
     "tsx_route.hip",
     "tsx_router.hip",
     "tsx_adapters.hip",
+    "tsx_adapters_back.hip",
     "tsx_prefill.hip",
 ]
 

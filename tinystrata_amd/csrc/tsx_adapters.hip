@@ -469,7 +469,7 @@ TSX_API int tsx_moe_adapters(const tsx_adapters* p, const int32_t* ids, const fl
     fill(k, p, ids, rows, t);
     k.x = x, k.ld_x = ld_x, k.base = base, k.ld_base = ld_base, k.y = y, k.ld_y = ld_y;
     const bool vec = matrix_quads(p) && quads(x, ld_x, 4);
-    k.cols = columns_per_block(t.plain, p->n_out, 128);
+    k.cols = columns_per_block((rows + 15) / 16, p->n_out, 128);
     const dim3 grid((unsigned) t.blocks(), (unsigned) ((p->n_out + k.cols - 1) / k.cols));
     const hipStream_t st = (hipStream_t) stream;
     if (p->type == TSX_F32) launch_rank<TSX_F32>(vec, k, grid, st);

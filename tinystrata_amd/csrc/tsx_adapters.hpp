@@ -21,9 +21,9 @@ constexpr int kMaxRank = 256;
 // one adapter (first: they have the ids to read before they know their rows), then the 16-row tiles as the rows stand.
 constexpr int kChunk = 4096, kMaxAdapters = 4096;
 struct Tiles {
-    int64_t plain;
+    int64_t plain;  // a multiple of 8: a run of tiles for each XCD
     int extra, chunks;
-    Tiles(int64_t rows, int n, int most) : plain((rows + 15) / 16), chunks((int) ((rows + kChunk - 1) / kChunk)) {
+    Tiles(int64_t rows, int n, int most) : plain((rows + 127) / 128 * 8), chunks((int) ((rows + kChunk - 1) / kChunk)) {
         // a class of c rows takes ceil(c / 16) tiles; there are at most n + 1 classes and as many as rows.  Past `most` of them
         // a block takes a further tile (a chunk of one adapter costs each of its blocks a look at the ids)
         const int64_t r = std::min<int64_t>(rows, kChunk);
@@ -43,15 +43,17 @@ __device__ __forceinline__ bool find_tile(Tile& t, const int32_t* ids, int64_t r
     static_assert(SEGS == 64, "one segment a lane");
     __shared__ int s_sum[WAVES], s_seg[SEGS], s_row[16], s_class, s_first;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    auto class_of = [&](int64_t j) {  // 0 .. n - 1, n for none, -1 past the rows
-        if (j >= rows) return -1;
-        const int id = ids[j];
-        return id < 0 || id >= n ? n : id;
+    auto class_of = [&](int64_t j) {  // 0 .. n - 1, n for none, -1 past the rows (an unconditional load: eight in flight)
+        const int id = ids[min(j, rows - 1)];
+        return j >= rows ? -1 : id < 0 || id >= n ? n : id;
     };
     if ((int) blockIdx.x >= regroup) {
         if (round > 0) return false;
-        t.row = ((int64_t) blockIdx.x - regroup) * 16 + (lane & 15);
+        // neighbouring tiles on one XCD (blocks go round them), whose L2 then holds the matrices of few adapters
+        const int q = blockIdx.x - regroup, per = (gridDim.x - regroup) / 8;
+        t.row = ((int64_t) (q % 8) * per + q / 8) * 16 + (lane & 15);
         const int c = class_of(t.row), first = __builtin_amdgcn_readfirstlane(c);
+        if (first < 0) return false;
         if (c < 0) t.row = -1;
         t.cur = first == n ? -1 : first;
         return __ballot(c >= 0 && c != first) == 0;
@@ -59,6 +61,33 @@ __device__ __forceinline__ bool find_tile(Tile& t, const int32_t* ids, int64_t r
     const int64_t base = (int64_t) (blockIdx.x / extra) * kChunk;
     const int mine = blockIdx.x % extra + round * extra;
     if (mine >= kChunk) return false;
+    if (rows <= 64) {
+        // a decode step: every wave has all rows on its lanes, and finds each lane's class mates from one ballot per bit of a
+        // class, with no barrier (64 mixed rows, 2048 -> 512, rank 16: 11.1 us, 15.0 the long way)
+        const int c = class_of(lane), lead = __shfl(c, lane & 48, 64);
+        const uint64_t other = __ballot(c >= 0 && c != lead), below = (1ull << lane) - 1;
+        const bool ours = c >= 0 && ((other >> (lane & 48)) & 0xFFFFu) != 0;
+        uint64_t mates = __ballot(ours);
+        if (!mates) return false;
+        for (int bit = 0; n >> bit; ++bit) {
+            const uint64_t set = __ballot(c >> bit & 1);
+            mates &= c >> bit & 1 ? set : ~set;
+        }
+        const int before = __builtin_popcountll(mates & below), k = (__builtin_popcountll(mates) + 15) / 16;
+        const bool leads = ours && before == 0;
+        int at = 0;  // tiles of the classes that a lower lane leads
+#pragma unroll
+        for (int q = 1; q <= 4; ++q) at += __builtin_popcountll(__ballot(leads && k >= q) & below);
+        const uint64_t hit = __ballot(leads && mine >= at && mine < at + k);
+        if (!hit) return false;
+        const int lane0 = __builtin_ctzll(hit), cls = __builtin_amdgcn_readlane(c, lane0);
+        const int to = before - 16 * (mine - __builtin_amdgcn_readlane(at, lane0));  // its place in the tile
+        const bool in = ours && c == cls && to >= 0 && to < 16;
+        const int got = __builtin_amdgcn_ds_permute(4 * (in ? to : 63), in ? lane + 1 : 0);  // 0 where none writes
+        t.row = (int64_t) __shfl(got, lane & 15, 64) - 1;
+        t.cur = cls == n ? -1 : cls;
+        return true;
+    }
     int c[R];
     bool some = false;
 #pragma unroll

@@ -430,7 +430,7 @@ TSX_API int tsx_moe_adapters_backward(const tsx_adapters* p, const int32_t* ids,
         k.v = sums && da ? v : nullptr;
         const bool vec = matrix_quads(p) && quads(x, ld_x, 4) && quads(dy, ld_dy, 4) && (!dx || quads(dx, ld_dx, 4)) &&
                          (!dbase || quads(dbase, ld_dbase, 4));
-        k.cols = dx ? columns_per_block(t.plain, p->n_in, 512) : p->n_in;
+        k.cols = dx ? columns_per_block((rows + 15) / 16, p->n_in, 512) : p->n_in;
         const dim3 grid((unsigned) t.blocks(), (unsigned) ((p->n_in + k.cols - 1) / k.cols));
         if (p->type == TSX_F32) launch_rank<TSX_F32>(vec, k, grid, st);
         else if (p->type == TSX_F16) launch_rank<TSX_F16>(vec, k, grid, st);

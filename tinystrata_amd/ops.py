@@ -27,8 +27,10 @@ def _p(t: torch.Tensor | None) -> int | None:
 
 
 def _stream(stream=None) -> int:
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+    if stream is not None:
+        return stream.cuda_stream
+    # the handle alone: torch.cuda.current_stream() makes an object first, 2.6 us of a call's 10
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 PLAIN_TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
@@ -42,14 +44,16 @@ def _expect(what: str, name: str, t: torch.Tensor | None, shape, dtype, like: to
         return
     if t.dtype != dtype:
         raise ValueError(f"{what}: {name} is {t.dtype}, not {dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, not {tuple(shape)}")
     if like is not None and t.device != like.device:
         raise ValueError(f"{what}: {name} is on {t.device}, not {like.device}")
+    if t.is_contiguous():
+        return
     if rows:
         if t.numel() and ((t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
             raise ValueError(f"{what}: {name}'s rows are not dense (strides {t.stride()})")
-    elif not t.is_contiguous():
+    else:
         raise ValueError(f"{what}: {name} is not contiguous")
 
 

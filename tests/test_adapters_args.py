@@ -54,8 +54,9 @@ def test_scratch_bytes():
     up = lambda v: (v + 255) // 256 * 256
     for rows, rank, pad in [(0, 16, 16), (5, 3, 16), (100, 33, 64), (4096, 100, 128), (7, 200, 256)]:
         a = args(rank=rank)
-        need = 2 * up(rows * pad * 4)
-        assert lib.tsx_moe_adapters_scratch_bytes(C.byref(a), rows) == need
+        uv, sums = 2 * up(rows * pad * 4), a.n * rank * (a.n_in + a.n_out) * 4     # and the sums of up to 16 parts of the rows
+        need = lib.tsx_moe_adapters_scratch_bytes(C.byref(a), rows)
+        assert need == uv or (need - uv) % sums == 0 and 2 <= (need - uv) // sums <= 16
     assert lib.tsx_moe_adapters_scratch_bytes(None, 5) == 0
     assert lib.tsx_moe_adapters_scratch_bytes(C.byref(args()), -1) == 0
 

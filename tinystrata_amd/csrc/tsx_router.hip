@@ -133,6 +133,11 @@ __device__ __forceinline__ float token_reduce(float v, Op op) {
     return v;
 }
 template <int L, int M = 1>
+__device__ __forceinline__ int token_count(int v) {
+    if constexpr (M < L) return token_count<L, 2 * M>(v + swap32<M>(v));
+    return v;
+}
+template <int L, int M = 1>
 __device__ __forceinline__ double token_sum(double v) {
     if constexpr (M < L) return token_sum<L, 2 * M>(v + swap64<M>(v));
     return v;
@@ -461,13 +466,15 @@ __global__ void __launch_bounds__(64 * WAVES) route_kernel(RouteArgs a) {
     bool picked = sub < a.k && mine > kNone;
     int id = picked ? key_id<kIdBits>(mine) : -1;
     if (a.bias) {
-        // the order of neighbours among the picks, and the last pick against what is left
+        // the order of neighbours among the picks, and the last pick against what is left: more values than picks that lie above
+        // it less its slack
         bool near = sub + 1 < a.k && next > kNone && mine - next <= 2.0 * slack(mine);
         const float cl = (float) last, edge = cl - 2.f * (float) slack(last);  // the id's bits round away
         const int el = key_id<kIdBits>(last);
+        int above = 0;
 #pragma unroll
-        for (int v = 0; v < V; ++v)
-            near |= kept && last > kNone && c[v] >= edge && (c[v] < cl || (c[v] == cl && p.e0 + p.pos(v) > el));
+        for (int v = 0; v < V; ++v) above += c[v] >= edge;
+        near |= last > kNone && token_count<L>(kept ? above : 0) > a.k;
         if (__any(near)) {
             if (sub + 1 < a.k && next > kNone && mine - next <= 2.0 * slack(mine)) {
                 const int e = key_id<kIdBits>(next);

@@ -228,7 +228,7 @@ TSX_API int tsx_moe_combine_norm(float* x, const float* parts, const int32_t* pr
  * The picks are those of exact arithmetic: c is formed in 64 bits.  prow (may be null) receives [n_tok][k] entry numbers
  * t * k + j, -1 where the id is -1: tsx_moe_combine's rows in entry order.  counts (may be null) has the number of tokens
  * that picked expert e added to counts[e].  n_expert 1..512, k 1..16, n_group 1..64 of equal size with k experts in those
- * kept; n_tok * k below 2^31.  tsx_moe_group and tsx_moe_route_sort leave out entries of id -1. */
+ * kept; n_tok * k below 2^31, n_tok below 2^26.  tsx_moe_group and tsx_moe_route_sort leave out entries of id -1. */
 enum { TSX_SCORE_SOFTMAX = 0, TSX_SCORE_SIGMOID = 1 };
 typedef struct {
     int32_t type;  /* of the logits: TSX_F32, TSX_F16 or TSX_BF16 */
@@ -250,7 +250,7 @@ TSX_API int tsx_moe_route_backward(const tsx_router* r, const void* logits, int6
  * dparts[p(t,j)] = wts[t][j] * dy[t], dshared[t] = g * dy[t] and dsgate[t] = g (1 - g) dy[t] . shared[t] with
  * g = sigmoid(sgate[t * sg_stride]).  Each of the four outputs may be null; dshared and dsgate go with shared.  dsgate is
  * dense.  The entries' rows are distinct; an entry without a row (prow below 0) has dwts 0, and rows of dparts that no entry
- * names are left as they are. */
+ * names are left as they are.  The outputs do not overlap dy or one another. */
 TSX_API int tsx_moe_combine_backward(const float* dy, const float* parts, const int32_t* prow, const float* wts, int k,
                                      const float* shared, const float* sgate, int sg_stride, int n, int n_tok,
                                      float* dwts, float* dparts, float* dshared, float* dsgate, void* stream);
@@ -323,7 +323,8 @@ typedef struct {
 } tsx_adapters;
 /* y[j] = base[j] + scale[a] * B_a (A_a x[j]) with a = ids[j], for `rows` rows of x (n_in floats, ld_x apart), base and y
  * (n_out floats); an id outside [0, n) is a row without an adapter: y[j] = base[j].  base may be y (rows without an adapter
- * are then not touched) or null (0).  The sums are in fp32.  One launch, no scratch; one token or many. */
+ * are then not touched) or null (0); y overlaps nothing else.  The sums are in fp32.  One launch, no scratch; one token or
+ * many. */
 TSX_API int tsx_moe_adapters(const tsx_adapters* p, const int32_t* ids, const float* x, int64_t ld_x, const float* base,
                              int64_t ld_base, float* y, int64_t ld_y, int64_t rows, void* stream);
 /* The gradients of tsx_moe_adapters from dy [rows][n_out]:
@@ -332,8 +333,8 @@ TSX_API int tsx_moe_adapters(const tsx_adapters* p, const int32_t* ids, const fl
  *   da[i] = sum over the rows of adapter i of v_j x[j]^T  (fp32 [n][rank][n_in]),
  *   db[i] = scale[i] * sum of dy[j] (A_i x[j])^T          (fp32 [n][n_out][rank]), both dense and written whole: 0 for an
  *           adapter without rows.  The sums' order depends on the ids alone.
- * Each of dx, da, db may be null.  scratch: tsx_moe_adapters_scratch_bytes(p, rows) bytes, 256-byte aligned,
- * nothing kept in it from one call for the next (calls that may overlap need one each). */
+ * Each of dx, da, db may be null; the outputs overlap nothing but dx its dbase.  scratch: tsx_moe_adapters_scratch_bytes(p,
+ * rows) bytes, 256-byte aligned, nothing kept in it from one call for the next (calls that may overlap need one each). */
 TSX_API size_t tsx_moe_adapters_scratch_bytes(const tsx_adapters* p, int64_t rows);
 TSX_API int tsx_moe_adapters_backward(const tsx_adapters* p, const int32_t* ids, const float* x, int64_t ld_x,
                                       const float* dy, int64_t ld_dy, const float* dbase, int64_t ld_dbase, float* dx,

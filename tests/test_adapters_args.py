@@ -81,3 +81,16 @@ def test_python_refusals():
                dict(dbase=torch.zeros(2, 32)), dict(scratch=torch.zeros(8, dtype=torch.uint8))]:
         with pytest.raises(ValueError, match=next(iter(kw))):
             ops.adapters_backward(ad, ids, x, y, **kw)
+
+
+def test_overlaps_and_grids_refused():
+    """Outputs in place of what other blocks read, and more threads than a launch counts."""
+    lib, a = _lib.lib(), args(n_in=32, n_out=32, a_stride=512)
+    for fn, good, changes in [(lib.tsx_moe_adapters, FORWARD, dict(x=(1, 1024), rows=(7, (1 << 31) - 1))),
+                              (lib.tsx_moe_adapters_backward, BACKWARD, dict(x=(1, 1024), dy=(3, 1024), rows=(11, 1 << 30)))]:
+        for name, (i, v) in changes.items():
+            b = list(good)
+            b[i] = v
+            assert fn(C.byref(a), *b) == _lib.TSX_ERR_ARG, name
+            said = lib.tsx_moe_last_error()
+            assert (b"too many rows" if name == "rows" else b"other blocks") in said, (name, said)

@@ -102,3 +102,18 @@ def test_python_refusals():
         args.update(kw)
         with pytest.raises(ValueError, match=name):
             ops.moe_combine_backward(dy, k=4, **args)
+
+
+def test_overlaps_and_grids_refused():
+    """The combine's gradient over its dy, and more threads than a launch counts."""
+    lib, a, e = _lib.lib(), router(k=1), _lib.TSX_ERR_ARG
+    for i, want in [(11, b"not overwritten"), (12, b"not overwritten")]:
+        args = [256, 512, None, 256, 8, 1024, 256, 1, 64, 1, 256, 2048, 4096, 256, None]
+        args[i] = 256
+        assert lib.tsx_moe_combine_backward(*args) == e and want in lib.tsx_moe_last_error()
+    args = [256, 512, None, 256, 8, 1024, 256, 1, 64, 1 << 30, 256, 2048, 4096, 256, None]
+    assert lib.tsx_moe_combine_backward(*args) == e and b"too many rows" in lib.tsx_moe_last_error()
+    assert lib.tsx_moe_route(C.byref(a), 256, 64, 256, 256, None, None, 1 << 26, None) == e
+    assert b"2^26" in lib.tsx_moe_last_error()
+    assert lib.tsx_moe_route_backward(C.byref(a), 256, 64, 256, 256, 256, 64, 1 << 28, None) == e
+    assert b"2^28" in lib.tsx_moe_last_error()

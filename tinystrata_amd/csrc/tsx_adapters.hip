@@ -21,8 +21,6 @@ namespace tsx {
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-
 
 template <int T> struct Elem { using type = uint16_t; };
 template <> struct Elem<TSX_F32> { using type = float; };
@@ -271,8 +269,8 @@ __device__ __forceinline__ bool sum_waves(const f32x4 (&acc)[RT], float s, int r
 // u of a tile: A x, summed and scaled.  Where the parts of x leave anything but numbers the fp32 instructions
 // are asked, which keep infinities apart from NaN
 template <int T, int RT, bool VEC>
-__device__ __forceinline__ void tile_u(float* u, const void* w, float s, int rank, const RowPair& x, int K, char* lds, char* own,
-                                       int wave, int lane, int turn) {
+__device__ __forceinline__ void tile_u(float* u, const void* w, float s, int rank, const RowPair& x, int K, char* lds,
+                                       char* own, int wave, int lane, int turn) {
     constexpr bool kSplit = T == TSX_BF16;
     {
         f32x4 acc[RT] = {};
@@ -348,7 +346,8 @@ struct OutRows {
 };
 
 template <int T, int RT, bool VEC>
-__global__ void __launch_bounds__((64 * Shape<T, RT>::kWaves)) __attribute__((amdgpu_waves_per_eu(RT <= (T == TSX_F32 ? 2 : 4) ? 4 : 1)))
+__global__ void __launch_bounds__((64 * Shape<T, RT>::kWaves))
+__attribute__((amdgpu_waves_per_eu(RT <= (T == TSX_F32 ? 2 : 4) ? 4 : 1)))
 adapters_kernel(AdArgs p) {
     using S = Shape<T, RT>;
     using E = elem_t<T>;
@@ -373,7 +372,7 @@ adapters_kernel(AdArgs p) {
             const int64_t first = __shfl(t.row, 0, 64);  // (every lane takes part)
             const int64_t at = t.row >= 0 ? t.row : first;
             tile_u<T, RT, VEC>(u, matrix_at<T>(p.a, t.cur * p.a_stride), p.scale ? p.scale[t.cur] : 1.f, p.rank,
-                                      RowPair(p.x, at, p.ld_x, lane), p.n_in, lds, own, wave, lane, (int) blockIdx.x * 5);
+                               RowPair(p.x, at, p.ld_x, lane), p.n_in, lds, own, wave, lane, (int) blockIdx.x * 5);
         }
         const UOperand<T, RT> uo(u, i, g);
         const OutRows rows(t.row, g);
@@ -464,12 +463,14 @@ TSX_API int tsx_moe_adapters(const tsx_adapters* p, const int32_t* ids, const fl
                 "tsx_moe_adapters: ids, x, y (and base) 4-byte aligned");
     TSX_REQUIRE(ld_x >= p->n_in && ld_y >= p->n_out && (!base || ld_base >= p->n_out) && (base != y || ld_base == ld_y),
                 "tsx_moe_adapters: rows as long as their columns; in place with one ld");
+    TSX_REQUIRE(y != x, "tsx_moe_adapters: x is read by other blocks than the one that writes y");
     AdArgs k{};
     const Tiles t(rows, p->n, 320);
     fill(k, p, ids, rows, t);
     k.x = x, k.ld_x = ld_x, k.base = base, k.ld_base = ld_base, k.y = y, k.ld_y = ld_y;
     const bool vec = matrix_quads(p) && quads(x, ld_x, 4);
     k.cols = columns_per_block((rows + 15) / 16, p->n_out, 128);
+    TSX_REQUIRE(grid_fits(t.blocks(), 512), "tsx_moe_adapters: too many rows");
     const dim3 grid((unsigned) t.blocks(), (unsigned) ((p->n_out + k.cols - 1) / k.cols));
     const hipStream_t st = (hipStream_t) stream;
     if (p->type == TSX_F32) launch_rank<TSX_F32>(vec, k, grid, st);

@@ -421,8 +421,8 @@ __global__ void __launch_bounds__(512) adapters_back_sum_kernel(AdSumArgs p) {
 }
 
 // the blocks that shared an adapter's rows, added up in their order
-__global__ void __launch_bounds__(256) adapters_back_join_kernel(const float* sums, int parts, int64_t apart, float* da, int64_t na,
-                                                                 float* db) {
+__global__ void __launch_bounds__(256) adapters_back_join_kernel(const float* sums, int parts, int64_t apart, float* da,
+                                                                 int64_t na, float* db) {
     const int64_t e = (int64_t) blockIdx.x * 256 + threadIdx.x;
     if (e >= apart) return;
     float t = sums[e];
@@ -460,7 +460,8 @@ inline size_t back_values(const tsx_adapters* p, int64_t rows) {
 inline int sum_parts(const tsx_adapters* p, int64_t rows) {
     if (p->n < 1 || p->n_in < 1 || p->n_out < 1) return 1;
     const int rt = sum_tiles(p->rank);
-    const int64_t blocks = (((int64_t) p->n_in + 63) / 64 + ((int64_t) p->n_out + 63) / 64) * p->n * ((p->rank + 16 * rt - 1) / (16 * rt));
+    const int64_t tiles = ((int64_t) p->n_in + 63) / 64 + ((int64_t) p->n_out + 63) / 64;
+    const int64_t blocks = tiles * p->n * ((p->rank + 16 * rt - 1) / (16 * rt));
     return (int) std::max<int64_t>(1, std::min<int64_t>({kSumBlocks / blocks, rows / p->n / kSumRows, 16}));
 }
 inline int64_t sum_values(const tsx_adapters* p) { return (int64_t) p->n * p->rank * ((int64_t) p->n_in + p->n_out); }
@@ -489,6 +490,8 @@ TSX_API int tsx_moe_adapters_backward(const tsx_adapters* p, const int32_t* ids,
     TSX_REQUIRE(rows == 0 || (ld_x >= p->n_in && ld_dy >= p->n_out && (!dx || ld_dx >= p->n_in) &&
                               (!dbase || ld_dbase >= p->n_in) && (!dbase || dbase != dx || ld_dbase == ld_dx)),
                 "tsx_moe_adapters_backward: rows as long as their columns; in place with one ld");
+    TSX_REQUIRE(!dx || (dx != x && dx != dy),
+                "tsx_moe_adapters_backward: x and dy are read by other blocks than those that write dx");
     const hipStream_t st = (hipStream_t) stream;
     float* u = (float*) scratch;
     float* v = u + back_values(p, rows);
@@ -496,6 +499,7 @@ TSX_API int tsx_moe_adapters_backward(const tsx_adapters* p, const int32_t* ids,
     if (rows) {
         AdArgs k{};
         const Tiles t(rows, p->n, INT32_MAX);
+        TSX_REQUIRE(grid_fits(t.blocks(), 512), "tsx_moe_adapters_backward: too many rows");
         fill(k, p, ids, rows, t);
         k.x = x, k.ld_x = ld_x, k.dy = dy, k.ld_dy = ld_dy, k.dbase = dbase, k.ld_dbase = ld_dbase, k.dx = dx, k.ld_dx = ld_dx;
         k.u = sums && db ? u : nullptr;

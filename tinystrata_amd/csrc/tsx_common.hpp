@@ -18,6 +18,9 @@ const char* error_cstr();
 // TSX_OK, or the launch's hipError_t with the message recorded
 int launch_status(const char* what);
 
+// a launch's threads are counted in 32 bits
+inline bool grid_fits(int64_t blocks, int threads) { return blocks <= (int64_t) UINT32_MAX / threads; }
+
 inline bool aligned(const void* p, uintptr_t a) { return ((uintptr_t) p % a) == 0; }
 
 // The current device's address of the no-allocation decode layer's scratch array (tsx_layer.hip); nullptr, with the

@@ -784,6 +784,7 @@ TSX_API int tsx_moe_route(const tsx_router* r, const void* logits, int64_t ld, i
                     aligned(prow, 4) && aligned(counts, 4),
                 "tsx_moe_route: logits, ids, weights (and prow, counts) aligned to their types");
     TSX_REQUIRE((int64_t) n_tok * r->k <= INT32_MAX, "tsx_moe_route: more than 2^31 - 1 entries");
+    TSX_REQUIRE(grid_fits(n_tok, 64), "tsx_moe_route: more than 2^26 - 1 tokens");
     RouteArgs a{};
     a.logits = logits, a.ld = ld, a.bias = r->bias, a.ids = ids, a.wts = weights, a.prow = prow, a.counts = counts;
     a.scale = r->scale, a.floor = r->floor;
@@ -830,6 +831,7 @@ TSX_API int tsx_moe_route_backward(const tsx_router* r, const void* logits, int6
     a.vec_in = r->n_expert % 4 == 0 && ld % 4 == 0 && aligned(logits, quad);
     a.vec_out = r->n_expert % 4 == 0 && ld_d % 4 == 0 && aligned(dlogits, quad);
     const unsigned blocks = (unsigned) (((int64_t) n_tok + 15) / 16);
+    TSX_REQUIRE(grid_fits(blocks, 256), "tsx_moe_route_backward: more than 2^28 - 16 tokens");
     const size_t lds = (size_t) 16 * ((r->n_expert + 3) & ~3) * 4;
     const hipStream_t st = (hipStream_t) stream;
     if (r->n_expert <= 64) route_back_kernel<4><<<blocks, 256, lds, st>>>(a);
@@ -853,7 +855,9 @@ TSX_API int tsx_moe_combine_backward(const float* dy, const float* parts, const 
     if (!(dwts || dparts || dshared || dsgate)) return TSX_OK;
     const int slots = k + (dshared || dsgate ? 1 : 0);
     const int64_t n_work = (int64_t) n_tok * slots, blocks = (n_work + 3) / 4;
-    TSX_REQUIRE(blocks <= INT32_MAX, "tsx_moe_combine_backward: too many rows");
+    TSX_REQUIRE(grid_fits(blocks, 256), "tsx_moe_combine_backward: too many rows");
+    TSX_REQUIRE(dparts != dy && dshared != dy,
+                "tsx_moe_combine_backward: dy is read by every entry of its token, not overwritten");
     const hipStream_t st = (hipStream_t) stream;
     if (n % 4 == 0 && aligned(dy, 16) && aligned(parts, 16) && aligned(shared, 16) && aligned(dparts, 16) &&
         aligned(dshared, 16))

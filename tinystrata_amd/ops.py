@@ -455,6 +455,8 @@ def adapters_backward(ad: Adapters, ids: torch.Tensor, x: torch.Tensor, dy: torc
     need = adapters_scratch_bytes(ad, rows)
     if scratch is None:
         scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
+        if stream is not None:
+            scratch.record_stream(stream)  # its memory goes back to the current stream's allocations when this returns
     elif scratch.device != x.device or not scratch.is_contiguous() or scratch.numel() * scratch.element_size() < need:
         raise ValueError(f"{what}: scratch of {need} bytes on {x.device} (adapters_scratch_bytes)")
     _launch(what, lib().tsx_moe_adapters_backward, x, stream, C.byref(ad.args), _p(ids), _p(x), _ld(x), _p(dy), _ld(dy),

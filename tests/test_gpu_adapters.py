@@ -273,3 +273,56 @@ def test_adapters_graph_and_repeat():
         out = [torch.empty_like(t) for t in (y, dx, da, db)]
         both(c, *out)
         assert all(torch.equal(p, q) for p, q in zip((y, dx, da, db), out)), k
+
+
+@pytest.mark.parametrize("n,rank,rows", [(1, 5, 600), (1, 24, 4600), (2, 60, 1500), (1, 130, 1100), (3, 16, 1700)])
+@pytest.mark.parametrize("vec", [True, False])
+def test_adapters_shared_sums(n, rank, rows, vec):
+    """Few adapters of many rows: blocks share an adapter's rows, for one gradient or both, with the same bits every time."""
+    c = make(n, rank, 72 if vec else 70, 132 if vec else 131, rows, "some", torch.float32, seed=rows)
+    ad = ops.Adapters(c["a"], c["b"], c["scale"])
+    pad = next(q for q in (16, 32, 64, 128, 256) if q >= rank)
+    assert ops.adapters_scratch_bytes(ad, rows) > 2 * (rows * pad * 4 + 256)  # more than u and v: the parts' sums
+    (_, da, db), (_, ma, mb) = backward_ref(c)
+    tol, seen = tolerance(c), {}
+    for want_a, want_b in [(True, True), (True, False), (False, True), (True, True)]:
+        ga = torch.full(ad.a.shape, 7.0, device="cuda") if want_a else None
+        gb = torch.full(ad.b.shape, 7.0, device="cuda") if want_b else None
+        ops.adapters_backward(ad, c["ids"], c["x"], c["dy"], da=ga, db=gb)
+        for name, g, want, mag in [("a", ga, da, ma), ("b", gb, db, mb)]:
+            if g is not None:
+                close(g, want, mag, tol)
+                assert torch.equal(seen.setdefault(name, g.clone()), g)
+
+
+@pytest.mark.parametrize("rows", [2, 3, 15, 17, 31, 48, 63, 64, 65])
+@pytest.mark.parametrize("n", [1, 2, 17, 4096])
+def test_adapters_decode_steps(rows, n):
+    """Mixed rows of a decode step, few and many to an adapter, more than 16 of one among them."""
+    c = make(n, 8, 40, 24, rows, "some", torch.bfloat16, seed=rows * 31 + n)
+    check(c)
+    c["ids"] = torch.where(torch.arange(rows, device="cuda") % 3 > 0, 0, c["ids"]).to(torch.int32)
+    check(c)
+
+
+def test_adapters_on_two_streams():
+    """Two calls at once on streams of their own, their scratch from the allocator."""
+    cs = [make(3, 16, 256, 320, 900, "some", torch.bfloat16, seed=s) for s in (1, 2)]
+    streams = [torch.cuda.Stream() for _ in cs]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(3):
+        for c, st in zip(cs, streams):
+            ad = ops.Adapters(c["a"], c["b"], c["scale"])
+            y, dx = torch.empty_like(c["base"]), torch.empty_like(c["x"])
+            da, db = (torch.empty(t.shape, device="cuda") for t in (ad.a, ad.b))
+            torch.cuda.synchronize()
+            ops.adapters(ad, c["ids"], c["x"], y, base=c["base"], stream=st)
+            ops.adapters_backward(ad, c["ids"], c["x"], c["dy"], dx=dx, da=da, db=db, dbase=c["dbase"], stream=st)
+            outs.append((c, y, dx, da, db))
+    torch.cuda.synchronize()
+    for c, y, *grads in outs:
+        want, mag = forward_ref(c)
+        close(y, want, mag, tolerance(c))
+        for got, want, mag in zip(grads, *backward_ref(c)):
+            close(got, want, mag, tolerance(c))

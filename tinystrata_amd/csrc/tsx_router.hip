@@ -7,9 +7,9 @@
 // the two largest s + bias) keep their experts.  The k largest c are picked, ties to the lower id.
 //
 // The order of the experts is that of exact arithmetic on the logits and biases given: two scores can lie nearer to each
-// other than their fp32 roundings (about one token in a thousand of a 16384 x 256 batch picks otherwise), so c is formed in
-// 64 bits where a bias or a sum enters it.  gfx950 issues 64-bit adds, products and maxima at the rate of 32-bit ones, so
-// this costs the polynomial of the exponential and no slower instructions.  The weights are in fp32.
+// other than their fp32 roundings (about one token in a thousand of a 16384 x 256 batch picks otherwise).  The choice is made on
+// fp32 values of known error, and made again in 64 bits where two values that decide it lie within that error (route_kernel).
+// The weights are in fp32.
 //
 // One fp64 key per expert holds c and, in its low 9 bits, the id (43 bits of c stay: two c that agree in them differ by less
 // than 2^-43 of their size), so that a maximum carries its id along and no two keys are equal.  A token belongs to L lanes;

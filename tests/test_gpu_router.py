@@ -363,3 +363,31 @@ def test_route_graph_and_stream():
     side.synchronize()
     b = ops.route(r, z[3])
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("E,k,seed", [(96, 6, 0), (256, 8, 0), (320, 16, 1)])
+@pytest.mark.parametrize("T", [1, 2050])
+@pytest.mark.parametrize("groups", [1, 8])
+def test_route_many_values_beyond_32_bits(E, k, seed, T, groups):
+    """Two thirds of the experts within 6e-8 of each other (the smallest gap is over 4e-13), among ordinary rows or alone; with
+    groups, those of a group, the groups well apart."""
+    rng = np.random.default_rng(seed)
+    z = rng.normal(0, 1, E).astype(np.float32)
+    s, _ = R.scores(z.astype(np.float64), "sigmoid")
+    bias = (1.25 - s).astype(np.float32)
+    bias[::3] -= np.float32(0.5)
+    c = np.sort((s + bias.astype(np.float64))[np.arange(E) % 3 > 0])
+    assert c[-1] - c[0] < 2e-7 and np.diff(c).min() > 4e-13
+    rows = rng.normal(0, 1, (T, E)).astype(np.float32)
+    rows[0] = rows[T // 2] = rows[T - 1] = z
+    rule = dict(score="sigmoid")
+    if groups > 1:
+        # a step of 2^-3 between groups: exact in the bias, so the gaps within a group stay
+        step = (np.float32(2) ** -3 * (np.arange(E) // (E // groups))).astype(np.float32)
+        shifted = (bias + step).astype(np.float32)
+        c = s + shifted.astype(np.float64)
+        for g in range(groups):
+            own = np.sort(c[g * E // groups:(g + 1) * E // groups])
+            assert np.diff(own).min() > 3e-13
+        bias, rule = shifted, dict(score="sigmoid", n_group=groups, topk_group=4, group_top=2)
+    check_route(dev(rows), k, bias, counts=True, prow=True, **rule)

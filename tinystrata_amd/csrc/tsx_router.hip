@@ -214,7 +214,7 @@ struct Place {
     }
     __device__ __forceinline__ int pos(int v) const { return 4 * (i + lanes * (v / 4)) + v % 4; }
 };
-// the lane's logits (-inf for one that takes no part), and biases
+// the lane's logits (-inf for one that takes no part), and biases; in quads without a condition, all in flight together
 template <int V>
 __device__ __forceinline__ void fetch_logits(const RouteArgs& a, const void* row, const Place& p, float (&l)[V]) {
 #pragma unroll
@@ -222,14 +222,14 @@ __device__ __forceinline__ void fetch_logits(const RouteArgs& a, const void* row
         const int pos = p.pos(4 * q);
         float o[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         if (a.vec) {
-            if (pos < p.size) logits4_at(row, a.type, p.e0 + pos, o);
+            logits4_at(row, a.type, pos < p.size ? p.e0 + pos : 0, o);
         } else {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
                 if (pos + c < p.size) o[c] = logit_at(row, a.type, p.e0 + pos + c);
         }
 #pragma unroll
-        for (int c = 0; c < 4; ++c) l[4 * q + c] = live_logit(o[c]);
+        for (int c = 0; c < 4; ++c) l[4 * q + c] = pos + c < p.size ? live_logit(o[c]) : -INFINITY;
     }
 }
 template <int V>
@@ -239,7 +239,7 @@ __device__ __forceinline__ void fetch_bias(const RouteArgs& a, const Place& p, f
         const int pos = p.pos(4 * q);
         float4 o = {0.f, 0.f, 0.f, 0.f};
         if (a.vec_bias) {
-            if (pos < p.size) o = *(const float4*) (a.bias + p.e0 + pos);
+            o = *(const float4*) (a.bias + (pos < p.size ? p.e0 + pos : 0));
         } else {
             if (pos < p.size) o.x = a.bias[p.e0 + pos];
             if (pos + 1 < p.size) o.y = a.bias[p.e0 + pos + 1];
@@ -357,7 +357,8 @@ __device__ __forceinline__ int pick_precise(const RouteArgs& a, const void* row,
 }
 
 // Choice values that need the scores are formed in fp32, from the hardware's exponential and reciprocal, and the selection is
-// made on them; only where two values that decide it lie within those roundings of each other is it made again in 64 bits.
+// made on them; only where two values that decide it lie within those roundings of each other is it made again in 64 bits: on
+// the few values near the last pick for a sigmoid, by pick_precise for a softmax and for the choice of groups.
 // `slack` bounds how far a value in fp32 is from the exact one.  A sigmoid: the exponential is off by 1.5 |l| + 2 units of
 // 2^-24, which s (1 - s) takes to less than 1, the sum with 1 and the reciprocal by 3; the sum with the bias by half a step of
 // at most 1 + |bias|: 5 + |bias| units in all.  A softmax: (2.5 |l - m| + 30) units of its size, |l - m| below 104 where it is
@@ -366,7 +367,8 @@ __device__ __forceinline__ int pick_precise(const RouteArgs& a, const void* row,
 //
 // Measured (us, sigmoid scores, bias, 8 groups by their two largest, top-8 of 256): 16384 tokens in 64 bits throughout 35.
 // Sixteen lanes a token or 64: one token 7.3 or 5.0, 2048 (no groups) 4.5 or 4.3, 4096 4.5 or 5.7, 16384 7.6 or 15.1; of 64
-// experts 2.6 or 3.4 at one token already.
+// experts 2.6 or 3.4 at one token already.  With values that leave doubt among them: 2048 tokens 8.2, 16384 18.1 (12.0 and 21.7
+// when pick_precise took every one); counts add 2.
 template <int L, int V, int K, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES) route_kernel(RouteArgs a) {
     extern __shared__ int s_count[];
@@ -476,9 +478,10 @@ __global__ void __launch_bounds__(64 * WAVES) route_kernel(RouteArgs a) {
         for (int v = 0; v < V; ++v) above += c[v] >= edge;
         near |= last > kNone && token_count<L>(kept ? above : 0) > a.k;
         if (__any(near)) {
+            bool doubt = false;
             if (sub + 1 < a.k && next > kNone && mine - next <= 2.0 * slack(mine)) {
                 const int e = key_id<kIdBits>(next);
-                open |= !(logit_at(row, a.type, id) == logit_at(row, a.type, e) && a.bias[id] == a.bias[e]);
+                doubt |= !(logit_at(row, a.type, id) == logit_at(row, a.type, e) && a.bias[id] == a.bias[e]);
             }
             if (kept && last > kNone) {
                 const float ll = logit_at(row, a.type, el), bl = a.bias[el];
@@ -487,8 +490,37 @@ __global__ void __launch_bounds__(64 * WAVES) route_kernel(RouteArgs a) {
                 fetch_bias<V>(a, p, b);
 #pragma unroll
                 for (int v = 0; v < V; ++v)
-                    open |= c[v] >= edge && (c[v] < cl || (c[v] == cl && p.e0 + p.pos(v) > el)) &&
-                            !(l[v] == ll && b[v] == bl);
+                    doubt |= c[v] >= edge && (c[v] < cl || (c[v] == cl && p.e0 + p.pos(v) > el)) &&
+                             !(l[v] == ll && b[v] == bl);
+            }
+            if (!a.sigmoid) {
+                open |= doubt;
+            } else if (__any(doubt)) {
+                // A sigmoid needs no sum over the experts: the values that reach the last pick less its slack, which hold
+                // every true pick, are formed in 64 bits (one or two a lane, as a rule) and merged again
+                uint32_t again = 0;
+#pragma unroll
+                for (int v = 0; v < V; ++v) again |= kept && c[v] > -INFINITY && c[v] >= edge ? 1u << v : 0u;
+#pragma unroll
+                for (int j = 0; j < K; ++j) top[j] = -INFINITY;
+#pragma unroll 1
+                while (__any(again != 0)) {
+                    double x = -INFINITY;
+                    if (again) {
+                        const int e = p.e0 + p.pos(__builtin_ctz(again));
+                        const double s = rcp64(1.0 + exp64(-(double) logit_at(row, a.type, e)));
+                        x = pack_key<kIdBits>(s + (double) a.bias[e], (uint32_t) e);
+                        again &= again - 1;
+                    }
+#pragma unroll
+                    for (int j = 0; j < K; ++j) sort_pair(top[j], x);
+                }
+                merge_lanes<L, K>(top);
+                mine = top[0];
+#pragma unroll
+                for (int j = 1; j < K; ++j) mine = sub == j ? top[j] : mine;
+                picked = sub < a.k && mine > kNone;
+                id = picked ? key_id<kIdBits>(mine) : -1;
             }
         }
     }

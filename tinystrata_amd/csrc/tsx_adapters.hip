@@ -188,7 +188,9 @@ __device__ __forceinline__ void contract_rows(f32x4 (&acc)[RT], const void* w, i
     using S = Shape<T, RT>;
     using E = elem_t<T>;
     constexpr int PIECE = 16 / S::kSize, PER = 32 / PIECE, LOADS = 16 * RT * PER / 64;  // 16-byte pieces a row, loads a chunk
-    constexpr int UN = RT == 1 ? 4 : RT <= 4 ? 2 : 1;
+    // chunks in flight besides the one that is multiplied: what four waves a SIMD leave registers for (rank 64, bf16, 4096 rows
+    // 2048 -> 1024 in segments: 27.1 us, with two 31.9; rank 16: 22.8, with one 25.6, with four 23.2)
+    constexpr int UN = RT == 1 ? 2 : 1;
     float* lx = (float*) lds;
     E* lw = (E*) (lds + S::kX);
     const int i = lane & 15, g = lane >> 4, col = lane % PER * PIECE;
@@ -378,7 +380,7 @@ adapters_kernel(AdArgs p) {
         const OutRows rows(t.row, g);
         const E* b = some ? (const E*) matrix_at<T>(p.b, t.cur * p.b_stride) : nullptr;
         // the block's columns 16 at a time: the wave's run of them, each column's ranks a row of LDS
-        constexpr int LOADS = 16 * 16 * RT / 4 / 64, UN = RT <= 2 ? 4 : 1;
+        constexpr int LOADS = 16 * 16 * RT / 4 / 64, UN = RT <= 2 ? 4 : RT <= 4 ? 2 : 1;
         using Four = four_t<T>;
         struct Reg {
             float old[4];

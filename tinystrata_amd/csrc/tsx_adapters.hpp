@@ -63,7 +63,7 @@ __device__ __forceinline__ bool find_tile(Tile& t, const int32_t* ids, int64_t r
     if (mine >= kChunk) return false;
     if (rows <= 64) {
         // a decode step: every wave has all rows on its lanes, and finds each lane's class mates from one ballot per bit of a
-        // class, with no barrier (64 mixed rows, 2048 -> 512, rank 16: 11.1 us, 15.0 the long way)
+        // class, with no barrier (64 mixed rows, 2048 -> 512, rank 16: 11.1 us for 15.0 the long way)
         const int c = class_of(lane), lead = __shfl(c, lane & 48, 64);
         const uint64_t other = __ballot(c >= 0 && c != lead), below = (1ull << lane) - 1;
         const bool ours = c >= 0 && ((other >> (lane & 48)) & 0xFFFFu) != 0;
